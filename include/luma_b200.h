@@ -43,7 +43,7 @@
 extern "C" {
 #endif
 
-#define LUMA_ABI_VERSION 4
+#define LUMA_ABI_VERSION 5
 
 /* Quantization grid constants (reference config.py:23-25). */
 #define LUMA_K_M 32767        /* signed int16 magnitude of Q_m        */
@@ -354,13 +354,97 @@ int luma_launch_config(int32_t* out, int n);
  */
 int luma_mc_copy(void* mc_dst, const void* src, uint64_t bytes, void* stream);
 
+/*
+ * Gradient operators: what runs between the backward pass and the step.  Each
+ * call takes a list of tensors as host arrays (read before the call returns)
+ * and works on all of them together.  Tensors may be of any size, 0 included,
+ * of mixed types and of any alignment that is a multiple of their element
+ * size; a tensor is `numel` consecutive elements.  Results are the same bits
+ * on every call with the same tensors.  No counterpart in the reference,
+ * whose loop clips with its framework's own functions (bench_nanogpt.py:
+ * 218-225).
+ *
+ * luma_grad_norm: the norm of all elements of all tensors.  With S the sum of
+ * x^2 (LUMA_NORM_2), the sum of |x| (LUMA_NORM_1) or the largest |x|
+ * (LUMA_NORM_MAX, NaN if any x is) over the elements x as stored, and c =
+ * *inv_scale, or 1:
+ *     r      = |c| * sqrt(S) (LUMA_NORM_2) or |c| * S
+ *     *norm  = r                        *coef = c * min(1, max_norm / (r + 1e-6))
+ *     *power = S                        norms[i] = sqrt(S_i) or S_i of tensor i
+ *     *found_inf = 1 if S is inf or NaN, that is if an element is
+ * each where the pointer is not NULL.  S is held in float64 (squares of
+ * elements are added in float32 within a few dozen elements, in float64 where
+ * that could overflow or lose them), r and the coefficient are computed in
+ * float64 and rounded once.
+ *
+ * luma_grad_finish: r, coef, norm, power and found_inf from `n_partials`
+ * values at `partials`, which are added (or whose maximum is taken): the
+ * second half of luma_grad_norm, for a `power` that was reduced over ranks.
+ *
+ * luma_grad_scale: x <- round(x * c) in place, c = host_scale * *scale (or
+ * host_scale); nothing is written when c == 1.
+ *
+ * luma_grad_clip: luma_grad_norm, then x <- round(x * *coef) in place
+ * (host_scale and scale are not used).
+ *
+ * luma_grad_accumulate: acc <- round(acc + c * x) (one fused multiply-add), or
+ * acc <- round(c * x) with overwrite != 0; accs are float32 or bfloat16.  With
+ * norm_kind != LUMA_NORM_NONE also the results of luma_grad_norm (norms
+ * excepted) for the accumulators as stored, from the same pass.
+ *
+ * Tensors that a call writes must not overlap one another, and a gradient may
+ * share memory with an accumulator only by being it; other lists are refused
+ * with LUMA_ERR_INVALID.
+ */
+enum {
+  LUMA_NORM_NONE = 0,
+  LUMA_NORM_1 = 1,
+  LUMA_NORM_2 = 2,
+  LUMA_NORM_MAX = 3
+};
+
+/* Doubles of workspace that a norm over n tensors needs. */
+#define LUMA_GRAD_TILES 16384
+#define LUMA_GRAD_PARTIALS(n) (LUMA_GRAD_TILES + 2 * (int64_t)(n))
+
+typedef struct LumaGradArgs {
+  const uint64_t* grads;      /* host [n]: device address of each tensor      */
+  const int64_t*  numel;      /* host [n]: its elements                       */
+  const uint8_t*  dtypes;     /* host [n]: LUMA_F32 | LUMA_BF16 | LUMA_F16    */
+  const uint64_t* accs;       /* host [n]: accumulators (accumulate only)     */
+  const uint8_t*  acc_dtypes; /* host [n]: LUMA_F32 | LUMA_BF16               */
+  int64_t         n;          /* tensors, at most 2^24                        */
+  double*         partials;   /* device workspace of this call, no contents
+                                 needed; calls that may overlap on the GPU
+                                 need one each                                */
+  int64_t         n_partials; /* its doubles, at least LUMA_GRAD_PARTIALS(n)  */
+  float*          norm;       /* device results, each may be NULL             */
+  float*          coef;
+  double*         power;
+  float*          norms;      /* device [n]                                   */
+  const float*    inv_scale;  /* device scalar or NULL                        */
+  float*          found_inf;  /* device flag or NULL: set to 1, never cleared */
+  const float*    scale;      /* device scalar or NULL                        */
+  double          max_norm;   /* 0 or more; used with coef                    */
+  float           host_scale;
+  int32_t         norm_kind;  /* LUMA_NORM_*                                  */
+  int32_t         overwrite;
+  int32_t         device;     /* CUDA device of the tensors and the stream    */
+} LumaGradArgs;
+
+int luma_grad_norm(const LumaGradArgs* args, void* stream);
+int luma_grad_finish(const LumaGradArgs* args, void* stream);
+int luma_grad_scale(const LumaGradArgs* args, void* stream);
+int luma_grad_clip(const LumaGradArgs* args, void* stream);
+int luma_grad_accumulate(const LumaGradArgs* args, void* stream);
+
 /* ABI version (LUMA_ABI_VERSION). */
 int luma_abi_version(void);
 
 /*
  * Layout check for FFI callers: writes sizeof of LumaTensorDesc, LumaStepRow,
- * LumaGrid, LumaSlot, LumaStepArgs into out[0..4] and returns 5 (or fewer if
- * n < 5).
+ * LumaGrid, LumaSlot, LumaStepArgs, LumaGradArgs into out[0..5] and returns 6
+ * (or n if n < 6).
  */
 int luma_struct_sizes(int64_t* out, int n);
 

@@ -10,6 +10,8 @@ from .optimizer import LUMA
 from . import torch_op  # registers torch.ops.luma_b200.step
 from .clip import clip_grad_coef
 from . import amp  # scaler_step: GradScaler.unscale_ fused into the step
+from .grads import accumulate_grads_, clip_coef, clip_grads_, grad_norm, scale_grads_
 
-__all__ = ["LUMA", "amp", "clip_grad_coef", "get_kernel_config", "K_M", "K_W", "SCALE_FLOOR_M"]
+__all__ = ["LUMA", "amp", "clip_grad_coef", "get_kernel_config", "K_M", "K_W", "SCALE_FLOOR_M",
+           "accumulate_grads_", "clip_coef", "clip_grads_", "grad_norm", "scale_grads_"]
 __version__ = "0.1.0"

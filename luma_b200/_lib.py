@@ -16,7 +16,7 @@ import numpy as np
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libluma_b200.so")
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 LUMA_OK = 0
 LUMA_ERR_INVALID = 1
@@ -79,14 +79,51 @@ class LumaStepArgs(ctypes.Structure):
     ]
 
 
+# norm kinds of the gradient operators, and the doubles of workspace they need
+NORM_NONE, NORM_1, NORM_2, NORM_MAX = 0, 1, 2, 3
+GRAD_TILES = 16384  # LUMA_GRAD_TILES
+
+
+def grad_partials(n: int) -> int:
+    """LUMA_GRAD_PARTIALS(n)."""
+    return GRAD_TILES + 2 * n
+
+
+class LumaGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("grads", ctypes.c_void_p),
+        ("numel", ctypes.c_void_p),
+        ("dtypes", ctypes.c_void_p),
+        ("accs", ctypes.c_void_p),
+        ("acc_dtypes", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("partials", ctypes.c_void_p),
+        ("n_partials", ctypes.c_int64),
+        ("norm", ctypes.c_void_p),
+        ("coef", ctypes.c_void_p),
+        ("power", ctypes.c_void_p),
+        ("norms", ctypes.c_void_p),
+        ("inv_scale", ctypes.c_void_p),
+        ("found_inf", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("max_norm", ctypes.c_double),
+        ("host_scale", ctypes.c_float),
+        ("norm_kind", ctypes.c_int32),
+        ("overwrite", ctypes.c_int32),
+        ("device", ctypes.c_int32),
+    ]
+
+
 EXPECTED_SIZES = (DESC_DTYPE.itemsize, ROW_DTYPE.itemsize, GRID_DTYPE.itemsize,
                   SLOT_DTYPE.itemsize, ctypes.sizeof(LumaStepArgs))
+EXPECTED_GRAD_SIZE = ctypes.sizeof(LumaGradArgs)
 
 EXPORTED = ("luma_step", "luma_step_noalloc", "luma_decode", "luma_quantize",
             "luma_abi_version", "luma_struct_sizes", "luma_last_error", "luma_arith_selfcheck",
             "luma_ipc_export", "luma_ipc_open", "luma_ipc_close", "luma_copy_async",
             "luma_error_flags", "luma_launch_config", "luma_mc_copy",
-            "luma_log_selfcheck")
+            "luma_log_selfcheck", *(f"luma_grad_{op}" for op in
+                                    ("norm", "finish", "scale", "clip", "accumulate")))
 
 KERR_ROW_RANGE = 1  # LUMA_KERR_ROW_RANGE
 
@@ -159,10 +196,15 @@ def lib() -> ctypes.CDLL:
         v = h.luma_abi_version()
         if v != ABI_VERSION:
             raise ImportError(f"libluma_b200 ABI {v}, expected {ABI_VERSION}")
-        sizes = (ctypes.c_int64 * 5)()
-        h.luma_struct_sizes(sizes, 5)
-        if tuple(sizes) != EXPECTED_SIZES:
-            raise ImportError(f"libluma_b200 struct sizes {tuple(sizes)} != {EXPECTED_SIZES}")
+        for op in ("norm", "finish", "scale", "clip", "accumulate"):
+            fn = getattr(h, f"luma_grad_{op}")
+            fn.restype = ctypes.c_int
+            fn.argtypes = [ctypes.POINTER(LumaGradArgs), ctypes.c_void_p]
+        sizes = (ctypes.c_int64 * 6)()
+        h.luma_struct_sizes(sizes, 6)
+        expected = (*EXPECTED_SIZES, EXPECTED_GRAD_SIZE)
+        if tuple(sizes) != expected:
+            raise ImportError(f"libluma_b200 struct sizes {tuple(sizes)} != {expected}")
         _lib = h
         return h
 

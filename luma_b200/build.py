@@ -15,7 +15,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = [os.path.join(HERE, "csrc", "luma_step.cu"), os.path.join(HERE, "csrc", "luma_peer.cu")]
+SOURCES = [os.path.join(HERE, "csrc", f"luma_{name}.cu") for name in ("step", "peer", "grad")]
 OUT = os.path.join(HERE, "_lib", "libluma_b200.so")
 
 NVCC_FLAGS = [

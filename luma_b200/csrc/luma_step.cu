@@ -2160,11 +2160,11 @@ int luma_launch_config(int32_t* out, int n) {
 }
 
 int luma_struct_sizes(int64_t* out, int n) {
-  const int64_t sizes[5] = {(int64_t)sizeof(LumaTensorDesc), (int64_t)sizeof(LumaStepRow),
+  const int64_t sizes[6] = {(int64_t)sizeof(LumaTensorDesc), (int64_t)sizeof(LumaStepRow),
                             (int64_t)sizeof(LumaGrid), (int64_t)sizeof(LumaSlot),
-                            (int64_t)sizeof(LumaStepArgs)};
+                            (int64_t)sizeof(LumaStepArgs), (int64_t)sizeof(LumaGradArgs)};
   if (out == nullptr || n <= 0) return 0;
-  const int k = n < 5 ? n : 5;
+  const int k = n < 6 ? n : 6;
   for (int i = 0; i < k; ++i) out[i] = sizes[i];
   return k;
 }

@@ -25,6 +25,7 @@ from torch.optim import Optimizer
 
 from . import _lib
 from .engine import Columns, DeviceEngine, Segment
+from .grads import clip_coef
 from .hostmath import SCALE_FLOOR_M, grid_record, precompute, rows_array, step_row, step_rows
 
 _BACKENDS = {"auto", "cuda", "triton"}
@@ -436,6 +437,17 @@ class LUMA(Optimizer):
             state.pop("S_v", None)
             if um is not None:
                 torch.cuda.current_stream(device).synchronize()  # injected draws outlive the kernel
+
+    # ------------------------------------------------------------------
+    # clipping
+    # ------------------------------------------------------------------
+    def clip_coef(self, max_norm: float, norm_type: float = 2.0,
+                  **kwargs) -> tuple[torch.Tensor, torch.Tensor]:
+        """(norm, coef) of this optimizer's gradients, for
+        ``step(grad_scale=coef)``: ``luma_b200.clip_coef`` (which documents the
+        further arguments) over every parameter that has a gradient."""
+        grads = [p.grad for g in self.param_groups for p in g["params"] if p.grad is not None]
+        return clip_coef(grads, max_norm, norm_type, **kwargs)
 
     # ------------------------------------------------------------------
     # step (optimizer.py:413-524)

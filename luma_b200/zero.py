@@ -52,6 +52,7 @@ from dataclasses import dataclass
 import torch
 
 from .engine import DeviceEngine, Segment
+from .grads import clip_coef, grad_norm
 from .hostmath import grid_record, rows_array, step_row
 
 ALIGN = 8
@@ -604,6 +605,34 @@ class ZeroLUMA:
                 if self.consumer is not None:
                     self.consumer(b, self.staging[b % n_st])
         main.wait_stream(comm)
+
+    def _grad_segments(self, grad_shard: torch.Tensor) -> list[torch.Tensor]:
+        """The parts of a grad shard that belong to tensors (the alignment gaps
+        and the last bucket's padding hold no gradients)."""
+        self._check(grad_shard)
+        return [grad_shard[sg.local:sg.local + sg.length] for sg in self.segments]
+
+    def _norm_group(self):
+        if self.layout.world == 1:
+            return None
+        import torch.distributed as dist
+        return self.pg if self.pg is not None else dist.group.WORLD
+
+    def grad_norm(self, grad_shard: torch.Tensor, norm_type: float = 2.0) -> torch.Tensor:
+        """Norm of the whole model's gradients, `grad_shard` being this rank's
+        (``luma_b200.grad_norm`` over every rank's segments; a collective)."""
+        with torch.cuda.device(self.flat.device):  # for a rank without segments
+            return grad_norm(self._grad_segments(grad_shard), norm_type,
+                             process_group=self._norm_group())
+
+    def clip_coef(self, grad_shard: torch.Tensor, max_norm: float,
+                  norm_type: float = 2.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """(norm, coef) of the whole model's gradients, the same on every rank,
+        for ``step(grad_shard, grad_scale=coef)`` (``luma_b200.clip_coef`` over
+        every rank's segments; a collective)."""
+        with torch.cuda.device(self.flat.device):
+            return clip_coef(self._grad_segments(grad_shard), max_norm, norm_type,
+                             process_group=self._norm_group())
 
     @torch.no_grad()
     def step_local(self, grad_shard: torch.Tensor,
