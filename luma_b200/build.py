@@ -1,4 +1,6 @@
-"""Build ``luma_b200/_lib/libluma_b200.so`` with nvcc for sm_100a.
+"""Build ``luma_b200/_lib/libluma_b200.so`` with nvcc for sm_100a, and the
+module ``luma_b200/_grads_ext.so`` (lists of torch tensors for the gradient
+operators) with g++ against the installed torch.
 
     python -m luma_b200.build [--debug]
 
@@ -12,11 +14,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SOURCES = [os.path.join(HERE, "csrc", f"luma_{name}.cu") for name in ("step", "peer", "grad")]
 OUT = os.path.join(HERE, "_lib", "libluma_b200.so")
+EXT_SOURCE = os.path.join(HERE, "csrc", "luma_torch.cpp")
+EXT_OUT = os.path.join(HERE, "_grads_ext.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -42,14 +47,35 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> str:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
     os.replace(OUT + ".tmp", OUT)
+    build_ext(verbose)
     return OUT
 
 
+def build_ext(verbose: bool = False) -> str:
+    """The torch-facing module; linked against the library and torch's own."""
+    import torch
+    from torch.utils import cpp_extension
+    libs = cpp_extension.library_paths("cuda")
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(ROOT, "include"),
+           *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")),
+           f"-isystem{sysconfig.get_paths()['include']}", EXT_SOURCE, "-o", EXT_OUT + ".tmp",
+           "-L", os.path.dirname(OUT), "-lluma_b200", *(f"-L{p}" for p in libs),
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN/_lib", *(f"-Wl,-rpath,{p}" for p in libs[:1])]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(EXT_OUT + ".tmp", EXT_OUT)
+    return EXT_OUT
+
+
 def is_stale() -> bool:
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(EXT_OUT):
         return True
-    t = os.path.getmtime(OUT)
-    deps = SOURCES + [os.path.join(ROOT, "include", "luma_b200.h"),
+    t = min(os.path.getmtime(OUT), os.path.getmtime(EXT_OUT))
+    deps = SOURCES + [EXT_SOURCE] + [os.path.join(ROOT, "include", "luma_b200.h"),
                       os.path.join(HERE, "csrc", "luma_internal.h")]
     return any(os.path.getmtime(s) > t for s in deps)
 

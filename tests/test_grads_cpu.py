@@ -12,7 +12,7 @@ from torch.amp.grad_scaler import OptState
 
 import luma_b200
 from luma_b200 import _lib, amp
-from luma_b200.grads import _dense, _List
+from luma_b200.grads import _ops
 
 from test_host_abi import _c_offsets
 
@@ -138,6 +138,8 @@ def test_refuses_what_is_no_dense_cuda_tensor(op):
         op([None])
     with pytest.raises(TypeError, match="float"):
         op([1.0])
+    with pytest.raises(TypeError, match="must be tensors"):
+        op(None)
     with pytest.raises(RuntimeError, match="sparse"):
         op([torch.zeros(4, 4).to_sparse()])
     with pytest.raises(ValueError, match="float64"):
@@ -187,13 +189,13 @@ def test_empty_lists():
 
 
 def test_dense_layouts():
+    _dense = _ops().dense
     x = torch.zeros(4, 6, 8)
     assert _dense(x.transpose(0, 2)) and _dense(x.permute(1, 2, 0))
     assert _dense(torch.zeros(2, 3, 4, 5).to(memory_format=torch.channels_last))
     assert _dense(torch.zeros(0, 3).t()) and _dense(torch.zeros(1).expand(1))
     assert not _dense(x[:, ::2]) and not _dense(x[:, :3]) and not _dense(torch.zeros(1).expand(5))
     assert not _dense(torch.zeros(3, 1).expand(3, 4)) and not _dense(torch.zeros(8).as_strided((4, 2), (1, 1)))
-    assert _List([], "grads").device is None
 
 
 # -- GradScaler ----------------------------------------------------------------
