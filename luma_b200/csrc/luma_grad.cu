@@ -28,7 +28,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTable = 1024;               // tensors per launch
-constexpr int64_t kMinTileElems = 1 << 14;
+constexpr int kVec = 32;                   // bytes of the widest load
+constexpr int kBatch = 4;                  // loads in flight per thread
+constexpr int64_t kMinTile = 1 << 15;      // bytes per tile: one batch of a CTA
 
 // Tensors of one launch.  Tile t belongs to the last entry i with
 // first[i] <= t; entries without elements have no tiles.
@@ -40,7 +42,7 @@ struct Table {
   uint8_t dtype[kTable];
   uint8_t src_dtype[kTable];
   int32_t n;
-  int64_t tile;            // elements per tile
+  int64_t tile;            // per tile: bytes, or elements in accumulate
 };
 
 struct FinishArgs {
@@ -64,24 +66,84 @@ __device__ __forceinline__ int find_entry(const Table& t, uint32_t tile) {
   return lo;
 }
 
-__device__ __forceinline__ float load_elem(uint64_t p, int dtype, int64_t i) {
-  if (dtype == LUMA_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == LUMA_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+// -- elements -----------------------------------------------------------------
+
+template <int DT> struct Elem { static constexpr int kSize = DT == LUMA_F32 ? 4 : 2; };
+
+template <int DT>
+__device__ __forceinline__ float to_float(uint32_t bits) {
+  if constexpr (DT == LUMA_F32) return __uint_as_float(bits);
+  else if constexpr (DT == LUMA_BF16) return __uint_as_float(bits << 16);
+  else return __half2float(__ushort_as_half((unsigned short)bits));
 }
 
-__device__ __forceinline__ void store_elem(uint64_t p, int dtype, int64_t i, float v) {
-  if (dtype == LUMA_F32) reinterpret_cast<float*>(p)[i] = v;
-  else if (dtype == LUMA_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+template <int DT>
+__device__ __forceinline__ uint32_t to_bits(float v) {
+  if constexpr (DT == LUMA_F32) return __float_as_uint(v);
+  else if constexpr (DT == LUMA_BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  else return __half_as_ushort(__float2half_rn(v));
 }
 
-// The value a store of v leaves behind.
-__device__ __forceinline__ float stored(int dtype, float v) {
-  if (dtype == LUMA_F32) return v;
-  if (dtype == LUMA_BF16) return __bfloat162float(__float2bfloat16_rn(v));
-  return __half2float(__float2half_rn(v));
+template <int DT>
+__device__ __forceinline__ float load_elem(const char* p) {
+  if constexpr (DT == LUMA_F32) return *reinterpret_cast<const float*>(p);
+  else return to_float<DT>(*reinterpret_cast<const uint16_t*>(p));
 }
+
+template <int DT>
+__device__ __forceinline__ void store_elem(char* p, float v) {
+  if constexpr (DT == LUMA_F32) *reinterpret_cast<float*>(p) = v;
+  else *reinterpret_cast<uint16_t*>(p) = (uint16_t)to_bits<DT>(v);
+}
+
+// The elements of a 32-bit word: one float32, or two 16-bit ones.
+template <int DT>
+__device__ __forceinline__ void unpack(uint32_t w, float* v) {
+  if constexpr (DT == LUMA_F32) {
+    v[0] = __uint_as_float(w);
+  } else if constexpr (DT == LUMA_BF16) {
+    v[0] = __uint_as_float(w << 16);
+    v[1] = __uint_as_float(w & 0xFFFF0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    v[0] = f.x;
+    v[1] = f.y;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack(const float* v) {
+  if constexpr (DT == LUMA_F32) {
+    return __float_as_uint(v[0]);
+  } else if constexpr (DT == LUMA_BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(v[0], v[1]);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+// 32 bytes read once: past L1, and from memory that nothing writes meanwhile.
+__device__ __forceinline__ void load_once(const char* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                 "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+
+__device__ __forceinline__ void load32(const char* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                 "=r"(w[6]), "=r"(w[7]) : "l"(p) : "memory");
+}
+
+__device__ __forceinline__ void store32(char* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                  "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+// -- sums ---------------------------------------------------------------------
 
 // max that keeps NaN, as the norm of a tensor with a NaN has to
 __device__ __forceinline__ double max_nan(double a, double b) {
@@ -97,6 +159,37 @@ __device__ __forceinline__ double power_of(int kind, float x) {
   return kind == LUMA_NORM_2 ? a * a : a;
 }
 
+// The powers of N elements joined onto `acc`: in float32, in four chains of
+// at most 16 additions, then in float64.  A float32 sum in [2^-100, 2^126] has
+// not overflowed, and what its squares lost below 2^-149 is less than 2^-40 of
+// it; a sum outside (all zeros excepted) is taken again in float64.  The
+// maximum is taken on the magnitudes' bits, whose order has NaN above inf.
+template <int KIND, int N>
+__device__ __forceinline__ double join_batch(double acc, const float (&v)[N]) {
+  if constexpr (KIND == LUMA_NORM_MAX) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return max_nan(acc, (double)__uint_as_float(m));
+  } else {
+    static_assert(N <= 64 && N % 4 == 0, "four chains of at most 16");
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      s[i & 3] = KIND == LUMA_NORM_2 ? fmaf(v[i], v[i], s[i & 3]) : s[i & 3] + fabsf(v[i]);
+    const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+    if (sum >= 0x1.0p-100f && sum <= 0x1.0p126f) return acc + (double)sum;
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) any |= __float_as_uint(v[i]);
+    if ((any & 0x7FFFFFFFu) != 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc += power_of(KIND, v[i]);
+    }
+    return acc;
+  }
+}
+
 // Result in thread 0.  Lanes and warps are joined in a fixed order.
 __device__ __forceinline__ double block_join(int kind, double v) {
   __shared__ double s[32];
@@ -109,15 +202,76 @@ __device__ __forceinline__ double block_join(int kind, double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kThreads) luma_grad_norm_kernel(
-    const __grid_constant__ Table t, int kind, double* partials) {
-  const int e = find_entry(t, blockIdx.x);
-  const int64_t lo = (int64_t)(blockIdx.x - t.first[e]) * t.tile;
-  const int64_t hi = min(lo + t.tile, t.numel[e]);
+// -- tiles of one tensor --------------------------------------------------------
+
+// Tiles of the norm and the scaling are cut at multiples of 32 bytes of the
+// address space, so that whatever a tensor's alignment all but its first and
+// last 32-byte line is read with full loads: [lo, hi) is the tensor's part of
+// a tile, [v0, v1) its full lines.
+struct Span {
+  char *lo, *hi, *v0, *v1;
+};
+
+template <int DT>
+__device__ __forceinline__ Span span_of(const Table& t, int e, uint32_t tile) {
+  const uint64_t p = t.ptr[e], end = p + (uint64_t)t.numel[e] * Elem<DT>::kSize;
+  const uint64_t from = (p & ~(uint64_t)(kVec - 1)) + (uint64_t)(tile - t.first[e]) * t.tile;
+  const uint64_t lo = max(p, from), hi = min(end, from + t.tile);
+  const uint64_t v0 = (lo + kVec - 1) & ~(uint64_t)(kVec - 1);
+  const uint64_t v1 = max(v0, hi & ~(uint64_t)(kVec - 1));
+  return {(char*)lo, (char*)hi, (char*)v0, (char*)v1};
+}
+
+// fn(address) for the elements outside the full lines: at most 30 of them, one
+// for each of the first threads.
+template <int DT, class F>
+__device__ __forceinline__ void for_edges(const Span& s, F&& fn) {
+  constexpr int kSize = Elem<DT>::kSize;
+  const int head = (int)(((s.v0 < s.hi ? s.v0 : s.hi) - s.lo) / kSize);
+  const int tail = s.hi > s.v1 ? (int)((s.hi - s.v1) / kSize) : 0;
+  const int i = threadIdx.x;
+  if (i < head) fn(s.lo + i * kSize);
+  else if (i < head + tail) fn(s.v1 + (i - head) * kSize);
+}
+
+template <int DT, int KIND>
+__device__ __forceinline__ double norm_tile(const Table& t, int e, uint32_t tile) {
+  constexpr int kPer = 4 / Elem<DT>::kSize;  // elements per word
+  const Span s = span_of<DT>(t, e, tile);
   double acc = 0.0;
-  for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads)
-    acc = join(kind, acc, power_of(kind, load_elem(t.ptr[e], t.dtype[e], i)));
-  acc = block_join(kind, acc);
+  for (const char* p = s.v0 + threadIdx.x * kVec; p < s.v1; p += kBatch * kThreads * kVec) {
+    uint32_t w[kBatch][8];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (p + u * kThreads * kVec < s.v1) {
+        load_once(p + u * kThreads * kVec, w[u]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[u][k] = 0;
+      }
+    }
+    float v[kBatch * 8 * kPer];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) unpack<DT>(w[u][k], v + (u * 8 + k) * kPer);
+    acc = join_batch<KIND>(acc, v);
+  }
+  for_edges<DT>(s, [&](const char* p) { acc = join(KIND, acc, power_of(KIND, load_elem<DT>(p))); });
+  return acc;
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) luma_grad_norm_kernel(
+    const __grid_constant__ Table t, double* partials) {
+  const int e = find_entry(t, blockIdx.x);
+  double acc;
+  switch (t.dtype[e]) {
+    case LUMA_F32: acc = norm_tile<LUMA_F32, KIND>(t, e, blockIdx.x); break;
+    case LUMA_BF16: acc = norm_tile<LUMA_BF16, KIND>(t, e, blockIdx.x); break;
+    default: acc = norm_tile<LUMA_F16, KIND>(t, e, blockIdx.x); break;
+  }
+  acc = block_join(KIND, acc);
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
 }
 
@@ -152,15 +306,48 @@ __global__ void __launch_bounds__(1024) luma_grad_finish_kernel(const FinishArgs
   }
 }
 
+template <int DT>
+__device__ __forceinline__ void scale_tile(const Table& t, int e, uint32_t tile, float c) {
+  constexpr int kPer = 4 / Elem<DT>::kSize;
+  const Span s = span_of<DT>(t, e, tile);
+  for (char* p = s.v0 + threadIdx.x * kVec; p < s.v1; p += kBatch * kThreads * kVec) {
+    uint32_t w[kBatch][8];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (p + u * kThreads * kVec < s.v1) load32(p + u * kThreads * kVec, w[u]);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (p + u * kThreads * kVec >= s.v1) break;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float v[kPer];
+        unpack<DT>(w[u][k], v);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) v[j] *= c;
+        w[u][k] = pack<DT>(v);
+      }
+      store32(p + u * kThreads * kVec, w[u]);
+    }
+  }
+  for_edges<DT>(s, [&](char* p) { store_elem<DT>(p, load_elem<DT>(p) * c); });
+}
+
 __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
     const __grid_constant__ Table t, float host_scale, const float* scale) {
   const float c = scale != nullptr ? host_scale * *scale : host_scale;
   if (c == 1.0f) return;  // x * 1 is x: nothing to write
   const int e = find_entry(t, blockIdx.x);
-  const int64_t lo = (int64_t)(blockIdx.x - t.first[e]) * t.tile;
-  const int64_t hi = min(lo + t.tile, t.numel[e]);
-  for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads)
-    store_elem(t.ptr[e], t.dtype[e], i, load_elem(t.ptr[e], t.dtype[e], i) * c);
+  switch (t.dtype[e]) {
+    case LUMA_F32: scale_tile<LUMA_F32>(t, e, blockIdx.x, c); break;
+    case LUMA_BF16: scale_tile<LUMA_BF16>(t, e, blockIdx.x, c); break;
+    default: scale_tile<LUMA_F16>(t, e, blockIdx.x, c); break;
+  }
+}
+
+__device__ __forceinline__ float load_any(uint64_t p, int dtype, int64_t i) {
+  if (dtype == LUMA_F32) return load_elem<LUMA_F32>((const char*)p + 4 * i);
+  if (dtype == LUMA_BF16) return load_elem<LUMA_BF16>((const char*)p + 2 * i);
+  return load_elem<LUMA_F16>((const char*)p + 2 * i);
 }
 
 __global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
@@ -172,10 +359,15 @@ __global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
   const int64_t hi = min(lo + t.tile, t.numel[e]);
   double acc = 0.0;
   for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-    const float g = load_elem(t.src[e], t.src_dtype[e], i);
-    const float v = overwrite ? c * g : fmaf(c, g, load_elem(t.ptr[e], t.dtype[e], i));
-    store_elem(t.ptr[e], t.dtype[e], i, v);
-    if (kind != LUMA_NORM_NONE) acc = join(kind, acc, power_of(kind, stored(t.dtype[e], v)));
+    const float g = load_any(t.src[e], t.src_dtype[e], i);
+    float v = overwrite ? c * g : fmaf(c, g, load_any(t.ptr[e], t.dtype[e], i));
+    if (t.dtype[e] == LUMA_F32) {
+      store_elem<LUMA_F32>((char*)t.ptr[e] + 4 * i, v);
+    } else {
+      store_elem<LUMA_BF16>((char*)t.ptr[e] + 2 * i, v);
+      v = to_float<LUMA_BF16>(to_bits<LUMA_BF16>(v));
+    }
+    if (kind != LUMA_NORM_NONE) acc = join(kind, acc, power_of(kind, v));
   }
   if (kind == LUMA_NORM_NONE) return;
   acc = block_join(kind, acc);
@@ -299,40 +491,40 @@ int check_disjoint(const char* what, const LumaGradArgs* a, const uint64_t* ptr,
   return LUMA_OK;
 }
 
-// Elements per tile: enough tiles to fill the GPU, at most about
-// LUMA_GRAD_TILES in all.
-int64_t tile_elems(const LumaGradArgs* a) {
+// Units (bytes, or elements in accumulate) per tile: at least one batch of a
+// CTA, and at most about LUMA_GRAD_TILES tiles in all.
+int64_t tile_size(const LumaGradArgs* a, bool elements) {
   double total = 0.0;
-  for (int64_t i = 0; i < a->n; ++i) total += (double)a->numel[i];
-  int64_t tile = kMinTileElems;
+  for (int64_t i = 0; i < a->n; ++i)
+    total += (double)a->numel[i] * (elements ? 1 : elem_size(a->dtypes[i]));
+  int64_t tile = elements ? kMinTile / 2 : kMinTile;
   while ((double)tile * LUMA_GRAD_TILES < total) tile *= 2;
   return tile;
 }
 
-int64_t tiles_of(int64_t numel, int64_t tile) { return (numel + tile - 1) / tile; }
-
 // Calls launch(table, index of its first tensor, its tiles, index of its first
-// tile) for every table of the call.
+// tile) for every table of the call.  Without `src` tiles are in bytes, from
+// the 32-byte line that the tensor begins in.
 template <class F>
 int for_tables(const LumaGradArgs* a, const uint64_t* ptr, const uint8_t* dtype,
                const uint64_t* src, const uint8_t* src_dtype, int64_t* n_tiles, F&& launch) {
   static thread_local Table t;
-  t.tile = tile_elems(a);
+  t.tile = tile_size(a, src != nullptr);
   int64_t done = 0;
   for (int64_t i = 0; i < a->n;) {
     const int64_t begin = i;
     int64_t tiles = 0;
     int k = 0;
     for (; i < a->n && k < kTable; ++i, ++k) {
-      const int64_t m = tiles_of(a->numel[i], t.tile);
-      if (tiles + m > 0x7FFFFFFF) break;
+      const int64_t units = src != nullptr || a->numel[i] == 0
+          ? a->numel[i] : a->numel[i] * elem_size(dtype[i]) + (int64_t)(ptr[i] % kVec);
       t.ptr[k] = ptr[i];
       t.src[k] = src != nullptr ? src[i] : 0;
       t.numel[k] = a->numel[i];
       t.dtype[k] = dtype[i];
       t.src_dtype[k] = src != nullptr ? src_dtype[i] : 0;
       t.first[k] = (uint32_t)tiles;
-      tiles += m;
+      tiles += (units + t.tile - 1) / t.tile;
     }
     t.first[k] = (uint32_t)tiles;
     t.n = k;
@@ -372,9 +564,12 @@ int norm_of(const LumaGradArgs* a, cudaStream_t st) {
   int64_t tiles_all = 0;
   int s = for_tables(a, a->grads, a->dtypes, nullptr, nullptr, &tiles_all,
                      [&](const Table& t, int64_t begin, int64_t tiles, int64_t first) {
-    if (tiles > 0)
-      luma_grad_norm_kernel<<<(unsigned)tiles, kThreads, 0, st>>>(t, a->norm_kind,
-                                                                  a->partials + first);
+    if (tiles > 0) {
+      auto* kernel = a->norm_kind == LUMA_NORM_1   ? luma_grad_norm_kernel<LUMA_NORM_1>
+                     : a->norm_kind == LUMA_NORM_2 ? luma_grad_norm_kernel<LUMA_NORM_2>
+                                                   : luma_grad_norm_kernel<LUMA_NORM_MAX>;
+      kernel<<<(unsigned)tiles, kThreads, 0, st>>>(t, a->partials + first);
+    }
     int r = launched("luma_grad_norm_kernel");
     if (r == LUMA_OK && a->norms != nullptr) {
       luma_grad_tensor_finish_kernel<<<(t.n + kWarps - 1) / kWarps, kThreads, 0, st>>>(
