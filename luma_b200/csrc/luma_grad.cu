@@ -344,34 +344,165 @@ __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
   }
 }
 
-__device__ __forceinline__ float load_any(uint64_t p, int dtype, int64_t i) {
-  if (dtype == LUMA_F32) return load_elem<LUMA_F32>((const char*)p + 4 * i);
-  if (dtype == LUMA_BF16) return load_elem<LUMA_BF16>((const char*)p + 2 * i);
-  return load_elem<LUMA_F16>((const char*)p + 2 * i);
+// Eight elements of consecutive memory, aligned to their size, as loaded.
+template <int DT> struct Eight { uint32_t w[DT == LUMA_F32 ? 8 : 4]; };
+
+template <int DT, bool ONCE>
+__device__ __forceinline__ Eight<DT> load8(const char* p) {
+  Eight<DT> x;
+  if constexpr (DT == LUMA_F32) {
+    if constexpr (ONCE) load_once(p, x.w); else load32(p, x.w);
+  } else if constexpr (ONCE) {
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]) : "l"(p));
+  } else {
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]) : "l"(p) : "memory");
+  }
+  return x;
 }
 
-__global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
-    const __grid_constant__ Table t, float host_scale, const float* scale, int overwrite, int kind,
-    double* partials) {
-  const float c = scale != nullptr ? host_scale * *scale : host_scale;
-  const int e = find_entry(t, blockIdx.x);
-  const int64_t lo = (int64_t)(blockIdx.x - t.first[e]) * t.tile;
-  const int64_t hi = min(lo + t.tile, t.numel[e]);
-  double acc = 0.0;
-  for (int64_t i = lo + threadIdx.x; i < hi; i += kThreads) {
-    const float g = load_any(t.src[e], t.src_dtype[e], i);
-    float v = overwrite ? c * g : fmaf(c, g, load_any(t.ptr[e], t.dtype[e], i));
-    if (t.dtype[e] == LUMA_F32) {
-      store_elem<LUMA_F32>((char*)t.ptr[e] + 4 * i, v);
-    } else {
-      store_elem<LUMA_BF16>((char*)t.ptr[e] + 2 * i, v);
-      v = to_float<LUMA_BF16>(to_bits<LUMA_BF16>(v));
-    }
-    if (kind != LUMA_NORM_NONE) acc = join(kind, acc, power_of(kind, v));
+template <int DT>
+__device__ __forceinline__ void unpack8(const Eight<DT>& x, float (&v)[8]) {
+  constexpr int kPer = 4 / Elem<DT>::kSize;
+#pragma unroll
+  for (int k = 0; k < 8 / kPer; ++k) unpack<DT>(x.w[k], v + k * kPer);
+}
+
+// Stores eight values; v becomes what was stored.
+template <int DT>
+__device__ __forceinline__ void store8(char* p, float (&v)[8]) {
+  constexpr int kPer = 4 / Elem<DT>::kSize;
+  Eight<DT> x;
+#pragma unroll
+  for (int k = 0; k < 8 / kPer; ++k) x.w[k] = pack<DT>(v + k * kPer);
+  if constexpr (DT == LUMA_F32) {
+    store32(p, x.w);
+  } else {
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};"
+                 :: "l"(p), "r"(x.w[0]), "r"(x.w[1]), "r"(x.w[2]), "r"(x.w[3]) : "memory");
+    unpack8<DT>(x, v);
   }
-  if (kind == LUMA_NORM_NONE) return;
-  acc = block_join(kind, acc);
-  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+}
+
+struct Accumulate {
+  float c;
+  bool overwrite;
+  __device__ __forceinline__ float operator()(float acc, float g) const {
+    return overwrite ? c * g : fmaf(c, g, acc);
+  }
+};
+
+// acc[lo, hi) of one tensor.  Where accumulator and gradient reach a multiple
+// of eight of their elements together, a thread works on eight consecutive
+// elements with one load each; elsewhere (a view at an odd offset) neighbouring
+// threads work on neighbouring elements.
+template <int AT, int GT, int KIND>
+__device__ __forceinline__ double accumulate_tile(const Table& t, int e, uint32_t tile,
+                                                  const Accumulate f) {
+  constexpr int kA = Elem<AT>::kSize, kG = Elem<GT>::kSize;
+  const int64_t n = t.numel[e];
+  char* const a0 = (char*)t.ptr[e];
+  const char* const g0 = (const char*)t.src[e];
+  int64_t lo = (int64_t)(tile - t.first[e]) * t.tile;
+  int64_t hi = min(lo + t.tile, n);
+  double sum = 0.0;
+  const auto one = [&](int64_t i) {
+    const float old = f.overwrite ? 0.0f : load_elem<AT>(a0 + i * kA);
+    float v = f(old, load_elem<GT>(g0 + i * kG));
+    store_elem<AT>(a0 + i * kA, v);
+    if constexpr (KIND != LUMA_NORM_NONE) {
+      v = to_float<AT>(to_bits<AT>(v));
+      sum = join(KIND, sum, power_of(KIND, v));
+    }
+  };
+  // elements before acc is at a multiple of eight elements
+  const int head = (int)((8 - (t.ptr[e] / kA) % 8) % 8);
+  if ((t.src[e] + (uint64_t)head * kG) % (8 * kG) == 0) {
+    lo = lo == 0 ? 0 : lo + head;  // tiles move with the alignment
+    hi = min(hi + head, n);
+    const int64_t v0 = lo == 0 ? min((int64_t)head, n) : min(lo, n);
+    const int64_t v1 = hi == n ? v0 + (max(hi - v0, (int64_t)0) & ~(int64_t)7) : hi;
+    for (int64_t i = v0 + threadIdx.x * 8; i < v1; i += kBatch * kThreads * 8) {
+      Eight<AT> x[kBatch];
+      Eight<GT> y[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int64_t j = i + u * kThreads * 8;
+        if (j < v1) {
+          if (!f.overwrite) x[u] = load8<AT, false>(a0 + j * kA);
+          y[u] = load8<GT, false>(g0 + j * kG);
+        }
+      }
+      float all[kBatch * 8];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int64_t j = i + u * kThreads * 8;
+        float v[8], g[8];
+        if (j < v1) {
+          unpack8<AT>(x[u], v);
+          unpack8<GT>(y[u], g);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[k] = f(v[k], g[k]);
+          store8<AT>(a0 + j * kA, v);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) all[u * 8 + k] = j < v1 ? v[k] : 0.0f;
+      }
+      if constexpr (KIND != LUMA_NORM_NONE) sum = join_batch<KIND>(sum, all);
+    }
+    const int64_t before = lo == 0 ? v0 : 0, behind = hi == n ? max(n - v1, (int64_t)0) : 0;
+    const int k = threadIdx.x;
+    if (k < before) one(k);
+    else if (k < before + behind) one(v1 + (k - before));
+  } else {
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * kThreads) {
+      float v[8], g[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t j = i + u * kThreads;
+        v[u] = g[u] = 0.0f;
+        if (j < hi) {
+          if (!f.overwrite) v[u] = load_elem<AT>(a0 + j * kA);
+          g[u] = load_elem<GT>(g0 + j * kG);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int64_t j = i + u * kThreads;
+        v[u] = f(v[u], g[u]);
+        if (j < hi) store_elem<AT>(a0 + j * kA, v[u]);
+        v[u] = j < hi ? to_float<AT>(to_bits<AT>(v[u])) : 0.0f;
+      }
+      if constexpr (KIND != LUMA_NORM_NONE) sum = join_batch<KIND>(sum, v);
+    }
+  }
+  return sum;
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
+    const __grid_constant__ Table t, float host_scale, const float* scale, int overwrite,
+    double* partials) {
+  const Accumulate f{scale != nullptr ? host_scale * *scale : host_scale, overwrite != 0};
+  const int e = find_entry(t, blockIdx.x);
+  double acc;
+  switch (t.dtype[e] * 4 + t.src_dtype[e]) {
+#define LUMA_CASE(A, G) \
+  case A * 4 + G: acc = accumulate_tile<A, G, KIND>(t, e, blockIdx.x, f); break;
+    LUMA_CASE(LUMA_F32, LUMA_F32)
+    LUMA_CASE(LUMA_F32, LUMA_BF16)
+    LUMA_CASE(LUMA_F32, LUMA_F16)
+    LUMA_CASE(LUMA_BF16, LUMA_F32)
+    LUMA_CASE(LUMA_BF16, LUMA_BF16)
+    LUMA_CASE(LUMA_BF16, LUMA_F16)
+#undef LUMA_CASE
+    default: return;  // the host lets no other types through
+  }
+  if constexpr (KIND != LUMA_NORM_NONE) {
+    acc = block_join(KIND, acc);
+    if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -675,10 +806,15 @@ int luma_grad_accumulate(const LumaGradArgs* a, void* stream) {
   int64_t tiles_all = 0;
   s = for_tables(a, a->accs, a->acc_dtypes, a->grads, a->dtypes, &tiles_all,
                  [&](const Table& t, int64_t, int64_t tiles, int64_t first) {
-    if (tiles > 0)
-      luma_grad_accumulate_kernel<<<(unsigned)tiles, kThreads, 0, st>>>(
-          t, a->host_scale, a->scale, a->overwrite, a->norm_kind,
-          a->partials != nullptr ? a->partials + first : nullptr);
+    if (tiles > 0) {
+      auto* kernel = a->norm_kind == LUMA_NORM_1   ? luma_grad_accumulate_kernel<LUMA_NORM_1>
+                     : a->norm_kind == LUMA_NORM_2 ? luma_grad_accumulate_kernel<LUMA_NORM_2>
+                     : a->norm_kind == LUMA_NORM_MAX ? luma_grad_accumulate_kernel<LUMA_NORM_MAX>
+                                                     : luma_grad_accumulate_kernel<LUMA_NORM_NONE>;
+      kernel<<<(unsigned)tiles, kThreads, 0, st>>>(t, a->host_scale, a->scale, a->overwrite,
+                                                   a->norm_kind != LUMA_NORM_NONE
+                                                       ? a->partials + first : nullptr);
+    }
     return launched("luma_grad_accumulate_kernel");
   });
   if (s == LUMA_OK && a->norm_kind != LUMA_NORM_NONE) s = finish(a, tiles_all, st);
