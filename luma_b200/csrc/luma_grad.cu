@@ -18,6 +18,7 @@
 #include <cmath>
 #include <cstdint>
 #include <mutex>
+#include <utility>
 #include <vector>
 
 #include "luma_b200.h"
@@ -26,7 +27,6 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kTable = 1024;               // tensors per launch
 constexpr int kVec = 32;                   // bytes of the widest load
 constexpr int kBatch = 4;                  // loads in flight per thread
@@ -56,6 +56,20 @@ struct FinishArgs {
   float* coef;
   double* power;
 };
+
+// The kernels of a call follow one another in a chain: each lets the next one
+// be set up on the SMs it leaves free (start_next), and the next one waits for
+// it to have ended, with all it wrote visible, before it touches what it needs
+// from it (wait_for_previous).  Every kernel of a chain waits before it ends,
+// so one that has ended has all before it behind it.  The first one is an
+// ordinary launch, for which the wait returns at once.
+__device__ __forceinline__ void start_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 __device__ __forceinline__ int find_entry(const Table& t, uint32_t tile) {
   int lo = 0, hi = t.n;  // first[lo] <= tile < first[hi]
@@ -264,6 +278,7 @@ __device__ __forceinline__ double norm_tile(const Table& t, int e, uint32_t tile
 template <int KIND>
 __global__ void __launch_bounds__(kThreads) luma_grad_norm_kernel(
     const __grid_constant__ Table t, double* partials) {
+  start_next();
   const int e = find_entry(t, blockIdx.x);
   double acc;
   switch (t.dtype[e]) {
@@ -273,25 +288,43 @@ __global__ void __launch_bounds__(kThreads) luma_grad_norm_kernel(
   }
   acc = block_join(KIND, acc);
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  wait_for_previous();  // the table before this one: other tensors, other partials
 }
 
-// One warp per tensor: its partials joined in order.
-__global__ void __launch_bounds__(kThreads) luma_grad_tensor_finish_kernel(
-    const __grid_constant__ Table t, int kind, const double* partials, float* norms) {
-  const int e = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (e >= t.n) return;
+// partials[0, n) joined by the CTA, result in thread 0.  Eight loads in flight
+// per thread: a chain of single ones costs a memory latency each (35 us of an
+// 80 us call for a tensor of 3,584 tiles).
+template <int THREADS>
+__device__ __forceinline__ double join_partials(int kind, const double* partials, int64_t n) {
   double acc = 0.0;
-  for (uint32_t k = t.first[e] + lane; k < t.first[e + 1]; k += 32)
-    acc = join(kind, acc, partials[k]);
+  for (int64_t i = threadIdx.x; i < n; i += 8 * THREADS) {
+    double v[8];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc = join(kind, acc, __shfl_down_sync(0xFFFFFFFFu, acc, o));
-  if (lane == 0) norms[e] = (float)(kind == LUMA_NORM_2 ? sqrt(acc) : acc);
+    for (int u = 0; u < 8; ++u)
+      v[u] = i + u * THREADS < n ? __ldcg(partials + i + u * THREADS) : 0.0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc = join(kind, acc, v[u]);
+  }
+  return block_join(kind, acc);
+}
+
+constexpr int kTensorThreads = 128;
+
+// One CTA per tensor.
+__global__ void __launch_bounds__(kTensorThreads) luma_grad_tensor_finish_kernel(
+    const __grid_constant__ Table t, int kind, const double* partials, float* norms) {
+  wait_for_previous();
+  start_next();
+  const int e = blockIdx.x;
+  const double acc = join_partials<kTensorThreads>(kind, partials + t.first[e],
+                                                   t.first[e + 1] - t.first[e]);
+  if (threadIdx.x == 0) norms[e] = (float)(kind == LUMA_NORM_2 ? sqrt(acc) : acc);
 }
 
 __global__ void __launch_bounds__(1024) luma_grad_finish_kernel(const FinishArgs a) {
-  double acc = 0.0;
-  for (int64_t i = threadIdx.x; i < a.n; i += 1024) acc = join(a.kind, acc, a.partials[i]);
-  acc = block_join(a.kind, acc);
+  wait_for_previous();
+  start_next();
+  const double acc = join_partials<1024>(a.kind, a.partials, a.n);
   if (threadIdx.x != 0) return;
   if (a.power != nullptr) *a.power = acc;
   // sums in 64 bits of finite float32 values are finite
@@ -334,7 +367,9 @@ __device__ __forceinline__ void scale_tile(const Table& t, int e, uint32_t tile,
 
 __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
     const __grid_constant__ Table t, float host_scale, const float* scale) {
-  const float c = scale != nullptr ? host_scale * *scale : host_scale;
+  wait_for_previous();
+  start_next();
+  const float c = scale != nullptr ? host_scale * __ldcg(scale) : host_scale;
   if (c == 1.0f) return;  // x * 1 is x: nothing to write
   const int e = find_entry(t, blockIdx.x);
   switch (t.dtype[e]) {
@@ -484,7 +519,8 @@ template <int KIND>
 __global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
     const __grid_constant__ Table t, float host_scale, const float* scale, int overwrite,
     double* partials) {
-  const Accumulate f{scale != nullptr ? host_scale * *scale : host_scale, overwrite != 0};
+  start_next();
+  const Accumulate f{scale != nullptr ? host_scale * __ldcg(scale) : host_scale, overwrite != 0};
   const int e = find_entry(t, blockIdx.x);
   double acc;
   switch (t.dtype[e] * 4 + t.src_dtype[e]) {
@@ -497,12 +533,13 @@ __global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
     LUMA_CASE(LUMA_BF16, LUMA_BF16)
     LUMA_CASE(LUMA_BF16, LUMA_F16)
 #undef LUMA_CASE
-    default: return;  // the host lets no other types through
+    default: acc = 0.0; break;  // the host lets no other types through
   }
   if constexpr (KIND != LUMA_NORM_NONE) {
     acc = block_join(KIND, acc);
     if (threadIdx.x == 0) partials[blockIdx.x] = acc;
   }
+  wait_for_previous();  // the table before this one: other tensors, other partials
 }
 
 // ---------------------------------------------------------------------------
@@ -667,16 +704,33 @@ int for_tables(const LumaGradArgs* a, const uint64_t* ptr, const uint8_t* dtype,
   return LUMA_OK;
 }
 
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? LUMA_OK : luma_cuda_fail(e, what);
-}
+// The launches of one call, in order on one stream.
+struct Chain {
+  cudaStream_t stream;
+  bool first = true;
 
-int finish(const LumaGradArgs* a, int64_t n_partials, cudaStream_t st) {
-  FinishArgs f{a->partials, n_partials, a->norm_kind, a->max_norm, a->inv_scale,
-               a->found_inf, a->norm, a->coef, a->power};
-  luma_grad_finish_kernel<<<1, 1024, 0, st>>>(f);
-  return launched("luma_grad_finish_kernel");
+  template <class... P, class... A>
+  int launch(const char* what, void (*kernel)(P...), int64_t grid, int threads, A&&... args) {
+    if (grid == 0) return LUMA_OK;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = first ? 0 : 1;
+    first = false;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+    return e == cudaSuccess ? LUMA_OK : luma_cuda_fail(e, what);
+  }
+};
+
+int finish(const LumaGradArgs* a, int64_t n_partials, Chain& chain) {
+  const FinishArgs f{a->partials, n_partials, a->norm_kind, a->max_norm, a->inv_scale,
+                     a->found_inf, a->norm, a->coef, a->power};
+  return chain.launch("luma_grad_finish_kernel", luma_grad_finish_kernel, 1, 1024, f);
 }
 
 int check_norm(const char* what, const LumaGradArgs* a) {
@@ -691,35 +745,30 @@ int check_norm(const char* what, const LumaGradArgs* a) {
   return LUMA_OK;
 }
 
-int norm_of(const LumaGradArgs* a, cudaStream_t st) {
+int norm_of(const LumaGradArgs* a, Chain& chain) {
+  auto* kernel = a->norm_kind == LUMA_NORM_1   ? luma_grad_norm_kernel<LUMA_NORM_1>
+                 : a->norm_kind == LUMA_NORM_2 ? luma_grad_norm_kernel<LUMA_NORM_2>
+                                               : luma_grad_norm_kernel<LUMA_NORM_MAX>;
   int64_t tiles_all = 0;
   int s = for_tables(a, a->grads, a->dtypes, nullptr, nullptr, &tiles_all,
                      [&](const Table& t, int64_t begin, int64_t tiles, int64_t first) {
-    if (tiles > 0) {
-      auto* kernel = a->norm_kind == LUMA_NORM_1   ? luma_grad_norm_kernel<LUMA_NORM_1>
-                     : a->norm_kind == LUMA_NORM_2 ? luma_grad_norm_kernel<LUMA_NORM_2>
-                                                   : luma_grad_norm_kernel<LUMA_NORM_MAX>;
-      kernel<<<(unsigned)tiles, kThreads, 0, st>>>(t, a->partials + first);
-    }
-    int r = launched("luma_grad_norm_kernel");
-    if (r == LUMA_OK && a->norms != nullptr) {
-      luma_grad_tensor_finish_kernel<<<(t.n + kWarps - 1) / kWarps, kThreads, 0, st>>>(
-          t, a->norm_kind, a->partials + first, a->norms + begin);
-      r = launched("luma_grad_tensor_finish_kernel");
-    }
+    int r = chain.launch("luma_grad_norm_kernel", kernel, tiles, kThreads, t,
+                         a->partials + first);
+    if (r == LUMA_OK && a->norms != nullptr)
+      r = chain.launch("luma_grad_tensor_finish_kernel", luma_grad_tensor_finish_kernel, t.n,
+                       kTensorThreads, t, a->norm_kind, a->partials + first, a->norms + begin);
     return r;
   });
-  if (s == LUMA_OK) s = finish(a, tiles_all, st);
+  if (s == LUMA_OK) s = finish(a, tiles_all, chain);
   return s;
 }
 
-int scale_of(const LumaGradArgs* a, float host_scale, const float* scale, cudaStream_t st) {
+int scale_of(const LumaGradArgs* a, float host_scale, const float* scale, Chain& chain) {
   int64_t tiles_all = 0;
   return for_tables(a, a->grads, a->dtypes, nullptr, nullptr, &tiles_all,
                     [&](const Table& t, int64_t, int64_t tiles, int64_t) {
-    if (tiles > 0)
-      luma_grad_scale_kernel<<<(unsigned)tiles, kThreads, 0, st>>>(t, host_scale, scale);
-    return launched("luma_grad_scale_kernel");
+    return chain.launch("luma_grad_scale_kernel", luma_grad_scale_kernel, tiles, kThreads, t,
+                        host_scale, scale);
   });
 }
 
@@ -742,7 +791,8 @@ int luma_grad_norm(const LumaGradArgs* a, void* stream) {
   if (s != LUMA_OK) return s;
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  return norm_of(a, static_cast<cudaStream_t>(stream));
+  Chain chain{static_cast<cudaStream_t>(stream)};
+  return norm_of(a, chain);
 }
 
 int luma_grad_finish(const LumaGradArgs* a, void* stream) {
@@ -759,7 +809,8 @@ int luma_grad_finish(const LumaGradArgs* a, void* stream) {
     return luma_fail(LUMA_ERR_INVALID, "luma_grad_finish: device %d", (int)a->device);
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  return finish(a, a->n_partials, static_cast<cudaStream_t>(stream));
+  Chain chain{static_cast<cudaStream_t>(stream)};
+  return finish(a, a->n_partials, chain);
 }
 
 int luma_grad_scale(const LumaGradArgs* a, void* stream) {
@@ -770,7 +821,8 @@ int luma_grad_scale(const LumaGradArgs* a, void* stream) {
   if (s != LUMA_OK) return s;
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  return scale_of(a, a->host_scale, a->scale, static_cast<cudaStream_t>(stream));
+  Chain chain{static_cast<cudaStream_t>(stream)};
+  return scale_of(a, a->host_scale, a->scale, chain);
 }
 
 int luma_grad_clip(const LumaGradArgs* a, void* stream) {
@@ -784,8 +836,9 @@ int luma_grad_clip(const LumaGradArgs* a, void* stream) {
   if (s != LUMA_OK) return s;
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  s = norm_of(a, static_cast<cudaStream_t>(stream));
-  if (s == LUMA_OK) s = scale_of(a, 1.0f, a->coef, static_cast<cudaStream_t>(stream));
+  Chain chain{static_cast<cudaStream_t>(stream)};
+  s = norm_of(a, chain);
+  if (s == LUMA_OK) s = scale_of(a, 1.0f, a->coef, chain);
   return s;
 }
 
@@ -802,22 +855,19 @@ int luma_grad_accumulate(const LumaGradArgs* a, void* stream) {
       return luma_fail(LUMA_ERR_INVALID, "%s: accumulator %lld is float16", what, (long long)i);
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto* kernel = a->norm_kind == LUMA_NORM_1     ? luma_grad_accumulate_kernel<LUMA_NORM_1>
+                 : a->norm_kind == LUMA_NORM_2   ? luma_grad_accumulate_kernel<LUMA_NORM_2>
+                 : a->norm_kind == LUMA_NORM_MAX ? luma_grad_accumulate_kernel<LUMA_NORM_MAX>
+                                                 : luma_grad_accumulate_kernel<LUMA_NORM_NONE>;
+  Chain chain{static_cast<cudaStream_t>(stream)};
   int64_t tiles_all = 0;
   s = for_tables(a, a->accs, a->acc_dtypes, a->grads, a->dtypes, &tiles_all,
                  [&](const Table& t, int64_t, int64_t tiles, int64_t first) {
-    if (tiles > 0) {
-      auto* kernel = a->norm_kind == LUMA_NORM_1   ? luma_grad_accumulate_kernel<LUMA_NORM_1>
-                     : a->norm_kind == LUMA_NORM_2 ? luma_grad_accumulate_kernel<LUMA_NORM_2>
-                     : a->norm_kind == LUMA_NORM_MAX ? luma_grad_accumulate_kernel<LUMA_NORM_MAX>
-                                                     : luma_grad_accumulate_kernel<LUMA_NORM_NONE>;
-      kernel<<<(unsigned)tiles, kThreads, 0, st>>>(t, a->host_scale, a->scale, a->overwrite,
-                                                   a->norm_kind != LUMA_NORM_NONE
-                                                       ? a->partials + first : nullptr);
-    }
-    return launched("luma_grad_accumulate_kernel");
+    return chain.launch("luma_grad_accumulate_kernel", kernel, tiles, kThreads, t, a->host_scale,
+                        a->scale, a->overwrite,
+                        a->norm_kind != LUMA_NORM_NONE ? a->partials + first : nullptr);
   });
-  if (s == LUMA_OK && a->norm_kind != LUMA_NORM_NONE) s = finish(a, tiles_all, st);
+  if (s == LUMA_OK && a->norm_kind != LUMA_NORM_NONE) s = finish(a, tiles_all, chain);
   return s;
 }
 
