@@ -13,6 +13,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <cooperative_groups.h>
 
 #include <algorithm>
 #include <cmath>
@@ -27,23 +28,40 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTable = 1024;               // tensors per launch
 constexpr int kVec = 32;                   // bytes of the widest load
 constexpr int kBatch = 4;                  // loads in flight per thread
-constexpr int64_t kMinTile = 1 << 15;      // bytes per tile: one batch of a CTA
+constexpr int kNormBatch = 2;              // of the norm, with five CTAs on an SM
+constexpr int kNormCtas = 5;
+// tiles: one batch of a CTA
+constexpr int64_t kNormTile = (int64_t)kNormBatch * kThreads * kVec;    // bytes
+constexpr int64_t kScaleTile = (int64_t)kBatch * kThreads * kVec;       // bytes
+constexpr int64_t kAccumulateTile = (int64_t)kBatch * kThreads * 8;     // elements
 
-// Tensors of one launch.  Tile t belongs to the last entry i with
+// Tensors of one launch, at most N.  Tile t belongs to the last entry i with
 // first[i] <= t; entries without elements have no tiles.
+template <int N>
 struct Table {
-  uint64_t ptr[kTable];
-  uint64_t src[kTable];    // accumulate: the gradient added to ptr
-  int64_t numel[kTable];
-  uint32_t first[kTable + 1];
-  uint8_t dtype[kTable];
-  uint8_t src_dtype[kTable];
+  static constexpr int kMost = N;
+  uint64_t ptr[N];
+  int64_t numel[N];
+  uint32_t first[N + 1];
+  uint8_t dtype[N];
   int32_t n;
-  int64_t tile;            // per tile: bytes, or elements in accumulate
+  int64_t tile;            // bytes per tile
 };
+
+// The same with the gradients that are added to ptr; tiles are in elements.
+template <int N>
+struct PairTable : Table<N> {
+  uint64_t src[N];
+  uint8_t src_dtype[N];
+};
+
+// A launch's parameters end at 32,764 bytes; calls with few tensors carry few.
+using Big = Table<1280>;
+using Small = Table<128>;
+using BigPair = PairTable<960>;
+using SmallPair = PairTable<128>;
 
 struct FinishArgs {
   const double* partials;
@@ -71,7 +89,8 @@ __device__ __forceinline__ void wait_for_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-__device__ __forceinline__ int find_entry(const Table& t, uint32_t tile) {
+template <class T>
+__device__ __forceinline__ int find_entry(const T& t, uint32_t tile) {
   int lo = 0, hi = t.n;  // first[lo] <= tile < first[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -209,6 +228,7 @@ __device__ __forceinline__ double block_join(int kind, double v) {
   __shared__ double s[32];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = join(kind, v, __shfl_down_sync(0xFFFFFFFFu, v, o));
+  __syncthreads();  // the call before is done with s
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x == 0)
@@ -221,71 +241,110 @@ __device__ __forceinline__ double block_join(int kind, double v) {
 // Tiles of the norm and the scaling are cut at multiples of 32 bytes of the
 // address space, so that whatever a tensor's alignment all but its first and
 // last 32-byte line is read with full loads: [lo, hi) is the tensor's part of
-// a tile, [v0, v1) its full lines.
+// the tiles [r0, r1), [v0, v1) its full lines.
 struct Span {
   char *lo, *hi, *v0, *v1;
 };
 
-template <int DT>
-__device__ __forceinline__ Span span_of(const Table& t, int e, uint32_t tile) {
+template <int DT, class T>
+__device__ __forceinline__ Span span_of(const T& t, int e, uint32_t r0, uint32_t r1) {
   const uint64_t p = t.ptr[e], end = p + (uint64_t)t.numel[e] * Elem<DT>::kSize;
-  const uint64_t from = (p & ~(uint64_t)(kVec - 1)) + (uint64_t)(tile - t.first[e]) * t.tile;
-  const uint64_t lo = max(p, from), hi = min(end, from + t.tile);
+  const uint64_t from = p & ~(uint64_t)(kVec - 1);
+  const uint64_t lo = max(p, from + (uint64_t)(r0 - t.first[e]) * t.tile);
+  const uint64_t hi = min(end, from + (uint64_t)(r1 - t.first[e]) * t.tile);
   const uint64_t v0 = (lo + kVec - 1) & ~(uint64_t)(kVec - 1);
   const uint64_t v1 = max(v0, hi & ~(uint64_t)(kVec - 1));
   return {(char*)lo, (char*)hi, (char*)v0, (char*)v1};
 }
 
 // fn(address) for the elements outside the full lines: at most 30 of them, one
-// for each of the first threads.
+// for each of the first threads of a team (`i` is the thread's place in it).
 template <int DT, class F>
-__device__ __forceinline__ void for_edges(const Span& s, F&& fn) {
+__device__ __forceinline__ void for_edges(const Span& s, int i, F&& fn) {
   constexpr int kSize = Elem<DT>::kSize;
   const int head = (int)(((s.v0 < s.hi ? s.v0 : s.hi) - s.lo) / kSize);
   const int tail = s.hi > s.v1 ? (int)((s.hi - s.v1) / kSize) : 0;
-  const int i = threadIdx.x;
   if (i < head) fn(s.lo + i * kSize);
   else if (i < head + tail) fn(s.v1 + (i - head) * kSize);
 }
 
-template <int DT, int KIND>
-__device__ __forceinline__ double norm_tile(const Table& t, int e, uint32_t tile) {
+// The powers of the tiles [r0, r1) joined onto `acc`, by a team of TEAM
+// threads.
+template <int DT, int KIND, int TEAM, class T>
+__device__ __forceinline__ double norm_tiles(const T& t, int e, uint32_t r0, uint32_t r1, int me,
+                                             double acc) {
   constexpr int kPer = 4 / Elem<DT>::kSize;  // elements per word
-  const Span s = span_of<DT>(t, e, tile);
-  double acc = 0.0;
-  for (const char* p = s.v0 + threadIdx.x * kVec; p < s.v1; p += kBatch * kThreads * kVec) {
-    uint32_t w[kBatch][8];
+  const Span s = span_of<DT>(t, e, r0, r1);
+#pragma unroll 1
+  for (const char* p = s.v0 + me * kVec; p < s.v1; p += kNormBatch * TEAM * kVec) {
+    uint32_t w[kNormBatch][8];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (p + u * kThreads * kVec < s.v1) {
-        load_once(p + u * kThreads * kVec, w[u]);
+    for (int u = 0; u < kNormBatch; ++u) {
+      if (p + u * TEAM * kVec < s.v1) {
+        // a team of one warp is luma_grad_small_kernel's, which may write later
+        if constexpr (TEAM == 32) load32(p + u * TEAM * kVec, w[u]);
+        else load_once(p + u * TEAM * kVec, w[u]);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[u][k] = 0;
       }
     }
-    float v[kBatch * 8 * kPer];
+    float v[kNormBatch * 8 * kPer];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
+    for (int u = 0; u < kNormBatch; ++u)
 #pragma unroll
       for (int k = 0; k < 8; ++k) unpack<DT>(w[u][k], v + (u * 8 + k) * kPer);
     acc = join_batch<KIND>(acc, v);
   }
-  for_edges<DT>(s, [&](const char* p) { acc = join(KIND, acc, power_of(KIND, load_elem<DT>(p))); });
+  for_edges<DT>(s, me, [&](const char* p) { acc = join(KIND, acc, power_of(KIND, load_elem<DT>(p))); });
   return acc;
 }
 
-template <int KIND>
-__global__ void __launch_bounds__(kThreads) luma_grad_norm_kernel(
-    const __grid_constant__ Table t, double* partials) {
-  start_next();
-  const int e = find_entry(t, blockIdx.x);
-  double acc;
+// The same by the tensor's type.
+template <int KIND, int TEAM, class T>
+__device__ __forceinline__ double norm_any(const T& t, int e, uint32_t r0, uint32_t r1, int me,
+                                           double acc) {
   switch (t.dtype[e]) {
-    case LUMA_F32: acc = norm_tile<LUMA_F32, KIND>(t, e, blockIdx.x); break;
-    case LUMA_BF16: acc = norm_tile<LUMA_BF16, KIND>(t, e, blockIdx.x); break;
-    default: acc = norm_tile<LUMA_F16, KIND>(t, e, blockIdx.x); break;
+    case LUMA_F32: return norm_tiles<LUMA_F32, KIND, TEAM>(t, e, r0, r1, me, acc);
+    case LUMA_BF16: return norm_tiles<LUMA_BF16, KIND, TEAM>(t, e, r0, r1, me, acc);
+    default: return norm_tiles<LUMA_F16, KIND, TEAM>(t, e, r0, r1, me, acc);
   }
+}
+
+// fn(entry, r0, r1) for the tiles of one of `teams` teams: an equal share of
+// all tiles of the table, one behind the other, entry by entry.
+template <class T, class F>
+__device__ __forceinline__ void for_share(const T& t, uint32_t team, uint32_t teams, F&& fn) {
+  const uint64_t tiles = t.first[t.n];
+  uint32_t r = (uint32_t)(tiles * team / teams);
+  const uint32_t end = (uint32_t)(tiles * (team + 1) / teams);
+  if (r == end) return;
+#pragma unroll 1
+  for (int e = find_entry(t, r); r < end; ++e) {
+    const uint32_t stop = min(end, t.first[e + 1]);
+    if (r < stop) fn(e, r, stop);
+    r = stop;
+  }
+}
+
+// fn(entry, r, r + 1) for every tile of one CTA, CTAs taking turns.
+template <class T, class F>
+__device__ __forceinline__ void for_turns(const T& t, F&& fn) {
+  const uint32_t tiles = t.first[t.n];
+#pragma unroll 1
+  for (uint32_t r = blockIdx.x; r < tiles; r += gridDim.x) fn(find_entry(t, r), r, r + 1);
+}
+
+// partials[CTA]: one for each CTA's share of the tiles, or where there are as
+// many CTAs as tiles one for each tile.
+template <int KIND, class T>
+__global__ void __launch_bounds__(kThreads, kNormCtas) luma_grad_norm_kernel(
+    const __grid_constant__ T t, double* partials) {
+  start_next();
+  double acc = 0.0;
+  for_share(t, blockIdx.x, gridDim.x, [&](int e, uint32_t r0, uint32_t r1) {
+    acc = norm_any<KIND, kThreads>(t, e, r0, r1, threadIdx.x, acc);
+  });
   acc = block_join(KIND, acc);
   if (threadIdx.x == 0) partials[blockIdx.x] = acc;
   wait_for_previous();  // the table before this one: other tensors, other partials
@@ -311,8 +370,9 @@ __device__ __forceinline__ double join_partials(int kind, const double* partials
 constexpr int kTensorThreads = 128;
 
 // One CTA per tensor.
+template <class T>
 __global__ void __launch_bounds__(kTensorThreads) luma_grad_tensor_finish_kernel(
-    const __grid_constant__ Table t, int kind, const double* partials, float* norms) {
+    const __grid_constant__ T t, int kind, const double* partials, float* norms) {
   wait_for_previous();
   start_next();
   const int e = blockIdx.x;
@@ -321,36 +381,48 @@ __global__ void __launch_bounds__(kTensorThreads) luma_grad_tensor_finish_kernel
   if (threadIdx.x == 0) norms[e] = (float)(kind == LUMA_NORM_2 ? sqrt(acc) : acc);
 }
 
+// One thread's work on the joined partials; returns the coefficient.
+__device__ __forceinline__ float write_results(const FinishArgs& a, double power) {
+  if (a.power != nullptr) *a.power = power;
+  // sums in 64 bits of finite float32 values are finite
+  if (a.found_inf != nullptr && !isfinite(power)) *a.found_inf = 1.0f;
+  const double inv = a.inv_scale != nullptr ? (double)*a.inv_scale : 1.0;
+  const double r = (a.kind == LUMA_NORM_2 ? sqrt(power) : power) * fabs(inv);
+  if (a.norm != nullptr) *a.norm = (float)r;
+  if (a.coef == nullptr) return 1.0f;
+  double c = a.max_norm / (r + 1e-6);
+  if (c > 1.0) c = 1.0;  // NaN stays NaN
+  *a.coef = (float)(c * inv);
+  return (float)(c * inv);
+}
+
 __global__ void __launch_bounds__(1024) luma_grad_finish_kernel(const FinishArgs a) {
   wait_for_previous();
   start_next();
   const double acc = join_partials<1024>(a.kind, a.partials, a.n);
-  if (threadIdx.x != 0) return;
-  if (a.power != nullptr) *a.power = acc;
-  // sums in 64 bits of finite float32 values are finite
-  if (a.found_inf != nullptr && !isfinite(acc)) *a.found_inf = 1.0f;
-  const double inv = a.inv_scale != nullptr ? (double)*a.inv_scale : 1.0;
-  const double r = (a.kind == LUMA_NORM_2 ? sqrt(acc) : acc) * fabs(inv);
-  if (a.norm != nullptr) *a.norm = (float)r;
-  if (a.coef != nullptr) {
-    double c = a.max_norm / (r + 1e-6);
-    if (c > 1.0) c = 1.0;  // NaN stays NaN
-    *a.coef = (float)(c * inv);
-  }
+  if (threadIdx.x == 0) write_results(a, acc);
 }
 
-template <int DT>
-__device__ __forceinline__ void scale_tile(const Table& t, int e, uint32_t tile, float c) {
+template <int DT, int TEAM, class T>
+__device__ __forceinline__ void scale_tiles(const T& t, int e, uint32_t r0, uint32_t r1, int me,
+                                            float c) {
   constexpr int kPer = 4 / Elem<DT>::kSize;
-  const Span s = span_of<DT>(t, e, tile);
-  for (char* p = s.v0 + threadIdx.x * kVec; p < s.v1; p += kBatch * kThreads * kVec) {
+  const Span s = span_of<DT>(t, e, r0, r1);
+#pragma unroll 1
+  for (char* p = s.v0 + me * kVec; p < s.v1; p += kBatch * TEAM * kVec) {
     uint32_t w[kBatch][8];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (p + u * kThreads * kVec < s.v1) load32(p + u * kThreads * kVec, w[u]);
+    for (int u = 0; u < kBatch; ++u) {
+      if (p + u * TEAM * kVec < s.v1) {
+        load32(p + u * TEAM * kVec, w[u]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[u][k] = 0;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      if (p + u * kThreads * kVec >= s.v1) break;
+      if (p + u * TEAM * kVec >= s.v1) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         float v[kPer];
@@ -359,24 +431,74 @@ __device__ __forceinline__ void scale_tile(const Table& t, int e, uint32_t tile,
         for (int j = 0; j < kPer; ++j) v[j] *= c;
         w[u][k] = pack<DT>(v);
       }
-      store32(p + u * kThreads * kVec, w[u]);
+      store32(p + u * TEAM * kVec, w[u]);
     }
   }
-  for_edges<DT>(s, [&](char* p) { store_elem<DT>(p, load_elem<DT>(p) * c); });
+  for_edges<DT>(s, me, [&](char* p) { store_elem<DT>(p, load_elem<DT>(p) * c); });
 }
 
+template <int TEAM, class T>
+__device__ __forceinline__ void scale_any(const T& t, int e, uint32_t r0, uint32_t r1, int me,
+                                          float c) {
+  switch (t.dtype[e]) {
+    case LUMA_F32: scale_tiles<LUMA_F32, TEAM>(t, e, r0, r1, me, c); break;
+    case LUMA_BF16: scale_tiles<LUMA_BF16, TEAM>(t, e, r0, r1, me, c); break;
+    default: scale_tiles<LUMA_F16, TEAM>(t, e, r0, r1, me, c); break;
+  }
+}
+
+template <class T>
 __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
-    const __grid_constant__ Table t, float host_scale, const float* scale) {
+    const __grid_constant__ T t, float host_scale, const float* scale) {
   wait_for_previous();
   start_next();
   const float c = scale != nullptr ? host_scale * __ldcg(scale) : host_scale;
   if (c == 1.0f) return;  // x * 1 is x: nothing to write
-  const int e = find_entry(t, blockIdx.x);
-  switch (t.dtype[e]) {
-    case LUMA_F32: scale_tile<LUMA_F32>(t, e, blockIdx.x, c); break;
-    case LUMA_BF16: scale_tile<LUMA_BF16>(t, e, blockIdx.x, c); break;
-    default: scale_tile<LUMA_F16>(t, e, blockIdx.x, c); break;
+  for_turns(t, [&](int e, uint32_t r0, uint32_t r1) {
+    scale_any<kThreads>(t, e, r0, r1, threadIdx.x, c);
+  });
+}
+
+// A small call as a whole: the norm, its results and with `clip` the scaling.
+// One cluster of eight CTAs whose warps share the tiles; the warps' sums are
+// joined in a fixed order, the CTAs' through distributed shared memory.
+constexpr int kClusterCtas = 8;
+constexpr int kClusterThreads = 1024;
+constexpr int64_t kWarpTile = (int64_t)kNormBatch * 32 * kVec;  // bytes
+
+template <int KIND>
+__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kClusterThreads)
+luma_grad_small_kernel(const __grid_constant__ Small t, const FinishArgs a, int clip) {
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  cg::cluster_group::arrival_token started = cluster.barrier_arrive();
+  __shared__ double sums[kClusterCtas];  // CTA 0's: one from each
+  __shared__ float coef;
+  constexpr uint32_t kWarps = kClusterThreads / 32;
+  // neighbouring warps of a CTA get tiles that lie next to one another
+  const uint32_t warp = blockIdx.x * kWarps + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  double acc = 0.0;
+  for_share(t, warp, kClusterCtas * kWarps, [&](int e, uint32_t r0, uint32_t r1) {
+    acc = norm_any<KIND, 32>(t, e, r0, r1, lane, acc);
+  });
+  acc = block_join(KIND, acc);
+  cluster.barrier_wait(std::move(started));  // every CTA has its shared memory
+  if (threadIdx.x == 0) *cluster.map_shared_rank(sums + blockIdx.x, 0) = acc;
+  cluster.sync();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    for (int k = 1; k < kClusterCtas; ++k) acc = join(KIND, acc, sums[k]);
+    const float c = write_results(a, acc);
+    if (clip)
+      for (int k = 0; k < kClusterCtas; ++k) *cluster.map_shared_rank(&coef, k) = c;
   }
+  if (!clip) return;
+  cluster.sync();
+  const float c = coef;
+  if (c == 1.0f) return;  // x * 1 is x: nothing to write
+  for_share(t, warp, kClusterCtas * kWarps, [&](int e, uint32_t r0, uint32_t r1) {
+    scale_any<32>(t, e, r0, r1, lane, c);
+  });
 }
 
 // Eight elements of consecutive memory, aligned to their size, as loaded.
@@ -428,20 +550,19 @@ struct Accumulate {
   }
 };
 
-// acc[lo, hi) of one tensor.  Where accumulator and gradient reach a multiple
+// The tiles [r0, r1) of one tensor.  Where accumulator and gradient reach a multiple
 // of eight of their elements together, a thread works on eight consecutive
 // elements with one load each; elsewhere (a view at an odd offset) neighbouring
 // threads work on neighbouring elements.
-template <int AT, int GT, int KIND>
-__device__ __forceinline__ double accumulate_tile(const Table& t, int e, uint32_t tile,
-                                                  const Accumulate f) {
+template <int AT, int GT, int KIND, class T>
+__device__ __forceinline__ double accumulate_tiles(const T& t, int e, uint32_t r0, uint32_t r1,
+                                                   const Accumulate f, double sum) {
   constexpr int kA = Elem<AT>::kSize, kG = Elem<GT>::kSize;
   const int64_t n = t.numel[e];
   char* const a0 = (char*)t.ptr[e];
   const char* const g0 = (const char*)t.src[e];
-  int64_t lo = (int64_t)(tile - t.first[e]) * t.tile;
-  int64_t hi = min(lo + t.tile, n);
-  double sum = 0.0;
+  int64_t lo = (int64_t)(r0 - t.first[e]) * t.tile;
+  int64_t hi = min((int64_t)(r1 - t.first[e]) * t.tile, n);
   const auto one = [&](int64_t i) {
     const float old = f.overwrite ? 0.0f : load_elem<AT>(a0 + i * kA);
     float v = f(old, load_elem<GT>(g0 + i * kG));
@@ -458,12 +579,15 @@ __device__ __forceinline__ double accumulate_tile(const Table& t, int e, uint32_
     hi = min(hi + head, n);
     const int64_t v0 = lo == 0 ? min((int64_t)head, n) : min(lo, n);
     const int64_t v1 = hi == n ? v0 + (max(hi - v0, (int64_t)0) & ~(int64_t)7) : hi;
+#pragma unroll 1
     for (int64_t i = v0 + threadIdx.x * 8; i < v1; i += kBatch * kThreads * 8) {
       Eight<AT> x[kBatch];
       Eight<GT> y[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const int64_t j = i + u * kThreads * 8;
+        x[u] = Eight<AT>{};
+        y[u] = Eight<GT>{};
         if (j < v1) {
           if (!f.overwrite) x[u] = load8<AT, false>(a0 + j * kA);
           y[u] = load8<GT, false>(g0 + j * kG);
@@ -474,13 +598,11 @@ __device__ __forceinline__ double accumulate_tile(const Table& t, int e, uint32_
       for (int u = 0; u < kBatch; ++u) {
         const int64_t j = i + u * kThreads * 8;
         float v[8], g[8];
-        if (j < v1) {
-          unpack8<AT>(x[u], v);
-          unpack8<GT>(y[u], g);
+        unpack8<AT>(x[u], v);
+        unpack8<GT>(y[u], g);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = f(v[k], g[k]);
-          store8<AT>(a0 + j * kA, v);
-        }
+        for (int k = 0; k < 8; ++k) v[k] = f(v[k], g[k]);
+        if (j < v1) store8<AT>(a0 + j * kA, v);
 #pragma unroll
         for (int k = 0; k < 8; ++k) all[u * 8 + k] = j < v1 ? v[k] : 0.0f;
       }
@@ -491,6 +613,7 @@ __device__ __forceinline__ double accumulate_tile(const Table& t, int e, uint32_
     if (k < before) one(k);
     else if (k < before + behind) one(v1 + (k - before));
   } else {
+#pragma unroll 1
     for (int64_t i = lo + threadIdx.x; i < hi; i += 8 * kThreads) {
       float v[8], g[8];
 #pragma unroll
@@ -515,26 +638,27 @@ __device__ __forceinline__ double accumulate_tile(const Table& t, int e, uint32_
   return sum;
 }
 
-template <int KIND>
+template <int KIND, class T>
 __global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
-    const __grid_constant__ Table t, float host_scale, const float* scale, int overwrite,
+    const __grid_constant__ T t, float host_scale, const float* scale, int overwrite,
     double* partials) {
   start_next();
   const Accumulate f{scale != nullptr ? host_scale * __ldcg(scale) : host_scale, overwrite != 0};
-  const int e = find_entry(t, blockIdx.x);
-  double acc;
-  switch (t.dtype[e] * 4 + t.src_dtype[e]) {
+  double acc = 0.0;
+  for_turns(t, [&](int e, uint32_t r0, uint32_t r1) {
+    switch (t.dtype[e] * 4 + t.src_dtype[e]) {
 #define LUMA_CASE(A, G) \
-  case A * 4 + G: acc = accumulate_tile<A, G, KIND>(t, e, blockIdx.x, f); break;
-    LUMA_CASE(LUMA_F32, LUMA_F32)
-    LUMA_CASE(LUMA_F32, LUMA_BF16)
-    LUMA_CASE(LUMA_F32, LUMA_F16)
-    LUMA_CASE(LUMA_BF16, LUMA_F32)
-    LUMA_CASE(LUMA_BF16, LUMA_BF16)
-    LUMA_CASE(LUMA_BF16, LUMA_F16)
+  case A * 4 + G: acc = accumulate_tiles<A, G, KIND>(t, e, r0, r1, f, acc); break;
+      LUMA_CASE(LUMA_F32, LUMA_F32)
+      LUMA_CASE(LUMA_F32, LUMA_BF16)
+      LUMA_CASE(LUMA_F32, LUMA_F16)
+      LUMA_CASE(LUMA_BF16, LUMA_F32)
+      LUMA_CASE(LUMA_BF16, LUMA_BF16)
+      LUMA_CASE(LUMA_BF16, LUMA_F16)
 #undef LUMA_CASE
-    default: acc = 0.0; break;  // the host lets no other types through
-  }
+      default: break;  // the host lets no other types through
+    }
+  });
   if constexpr (KIND != LUMA_NORM_NONE) {
     acc = block_join(KIND, acc);
     if (threadIdx.x == 0) partials[blockIdx.x] = acc;
@@ -548,9 +672,11 @@ __global__ void __launch_bounds__(kThreads) luma_grad_accumulate_kernel(
 
 constexpr int kMaxDevices = 64;
 
-// 0: not looked at yet, 1: usable, 2: another architecture
+// What is known of each device: 0 nothing yet, 1 usable, 2 another
+// architecture; and the CTAs it holds at once of each kernel.
 int g_usable[kMaxDevices];
-std::mutex g_usable_mu;
+std::vector<std::pair<const void*, int>> g_resident[kMaxDevices];
+std::mutex g_devices_mu;
 
 // Makes a device current for one call and puts the caller's back.
 struct DeviceScope {
@@ -571,7 +697,7 @@ struct DeviceScope {
       status = luma_fail(LUMA_ERR_INVALID, "device index %d out of range", dev);
       return;
     }
-    std::lock_guard<std::mutex> lk(g_usable_mu);
+    std::lock_guard<std::mutex> lk(g_devices_mu);
     if (g_usable[dev] == 0) {
       int major = 0;
       e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
@@ -659,55 +785,98 @@ int check_disjoint(const char* what, const LumaGradArgs* a, const uint64_t* ptr,
   return LUMA_OK;
 }
 
-// Units (bytes, or elements in accumulate) per tile: at least one batch of a
-// CTA, and at most about LUMA_GRAD_TILES tiles in all.
-int64_t tile_size(const LumaGradArgs* a, bool elements) {
-  double total = 0.0;
-  for (int64_t i = 0; i < a->n; ++i)
-    total += (double)a->numel[i] * (elements ? 1 : elem_size(a->dtypes[i]));
-  int64_t tile = elements ? kMinTile / 2 : kMinTile;
-  while ((double)tile * LUMA_GRAD_TILES < total) tile *= 2;
+// A tile's size: `least`, or more where that would give more than `most` tiles.
+int64_t tile_size(double total, int64_t least, int64_t most) {
+  int64_t tile = least;
+  while ((double)tile * (double)most < total) tile *= 2;
   return tile;
 }
 
-// Calls launch(table, index of its first tensor, its tiles, index of its first
-// tile) for every table of the call.  Without `src` tiles are in bytes, from
-// the 32-byte line that the tensor begins in.
-template <class F>
-int for_tables(const LumaGradArgs* a, const uint64_t* ptr, const uint8_t* dtype,
-               const uint64_t* src, const uint8_t* src_dtype, int64_t* n_tiles, F&& launch) {
-  static thread_local Table t;
-  t.tile = tile_size(a, src != nullptr);
-  int64_t done = 0;
+// At most about LUMA_GRAD_TILES where tiles have a partial each; elsewhere
+// their number only has to stay within 32 bits.
+constexpr int64_t kManyTiles = (int64_t)1 << 30;
+
+double total_bytes(const LumaGradArgs* a) {
+  double total = 0.0;
+  for (int64_t i = 0; i < a->n; ++i) total += (double)a->numel[i] * elem_size(a->dtypes[i]);
+  return total;
+}
+
+// Fills an entry and returns its tiles.  Norm and scaling: from the 32-byte
+// line that the tensor begins in.
+template <int N>
+int64_t fill(Table<N>& t, int k, const LumaGradArgs* a, int64_t i) {
+  t.ptr[k] = a->grads[i];
+  t.numel[k] = a->numel[i];
+  t.dtype[k] = a->dtypes[i];
+  if (a->numel[i] == 0) return 0;
+  const int64_t bytes = a->numel[i] * elem_size(a->dtypes[i]) + (int64_t)(a->grads[i] % kVec);
+  return (bytes + t.tile - 1) / t.tile;
+}
+
+template <int N>
+int64_t fill(PairTable<N>& t, int k, const LumaGradArgs* a, int64_t i) {
+  t.ptr[k] = a->accs[i];
+  t.numel[k] = a->numel[i];
+  t.dtype[k] = a->acc_dtypes[i];
+  t.src[k] = a->grads[i];
+  t.src_dtype[k] = a->dtypes[i];
+  return (a->numel[i] + t.tile - 1) / t.tile;
+}
+
+// Calls launch(table, index of its first tensor, its tiles) for every table of
+// the call.
+template <class T, class F>
+int for_tables(const LumaGradArgs* a, int64_t tile, F&& launch) {
+  static thread_local T t;
+  t.tile = tile;
   for (int64_t i = 0; i < a->n;) {
     const int64_t begin = i;
     int64_t tiles = 0;
     int k = 0;
-    for (; i < a->n && k < kTable; ++i, ++k) {
-      const int64_t units = src != nullptr || a->numel[i] == 0
-          ? a->numel[i] : a->numel[i] * elem_size(dtype[i]) + (int64_t)(ptr[i] % kVec);
-      t.ptr[k] = ptr[i];
-      t.src[k] = src != nullptr ? src[i] : 0;
-      t.numel[k] = a->numel[i];
-      t.dtype[k] = dtype[i];
-      t.src_dtype[k] = src != nullptr ? src_dtype[i] : 0;
+    for (; i < a->n && k < T::kMost; ++i, ++k) {
       t.first[k] = (uint32_t)tiles;
-      tiles += (units + t.tile - 1) / t.tile;
+      tiles += fill(t, k, a, i);
     }
     t.first[k] = (uint32_t)tiles;
     t.n = k;
-    const int st = launch(t, begin, tiles, done);
+    const int st = launch(t, begin, tiles);
     if (st != LUMA_OK) return st;
-    done += tiles;
   }
-  *n_tiles = done;
   return LUMA_OK;
 }
 
 // The launches of one call, in order on one stream.
 struct Chain {
+  int device;
   cudaStream_t stream;
   bool first = true;
+
+  Chain(int dev, void* st) : device(dev), stream(static_cast<cudaStream_t>(st)) {}
+
+  // CTAs for so many tiles: at most what the device holds at once of a kernel.
+  template <class K>
+  int64_t grid(K* kernel, int64_t tiles) {
+    int64_t most = 0;
+    {
+      std::lock_guard<std::mutex> lk(g_devices_mu);
+      std::vector<std::pair<const void*, int>>& known = g_resident[device];
+      for (const auto& [k, n] : known)
+        if (k == (const void*)kernel) most = n;
+      if (most == 0) {
+        int sms = 0, per = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, 0) !=
+                cudaSuccess || sms * per == 0) {
+          cudaGetLastError();
+          sms = 148, per = 1;  // a guess is as right, only slower
+        }
+        most = sms * per;
+        known.emplace_back((const void*)kernel, (int)most);
+      }
+    }
+    return std::min(tiles, most);
+  }
 
   template <class... P, class... A>
   int launch(const char* what, void (*kernel)(P...), int64_t grid, int threads, A&&... args) {
@@ -727,10 +896,14 @@ struct Chain {
   }
 };
 
+FinishArgs finish_args(const LumaGradArgs* a, int64_t n_partials) {
+  return {a->partials, n_partials, a->norm_kind, a->max_norm, a->inv_scale,
+          a->found_inf, a->norm, a->coef, a->power};
+}
+
 int finish(const LumaGradArgs* a, int64_t n_partials, Chain& chain) {
-  const FinishArgs f{a->partials, n_partials, a->norm_kind, a->max_norm, a->inv_scale,
-                     a->found_inf, a->norm, a->coef, a->power};
-  return chain.launch("luma_grad_finish_kernel", luma_grad_finish_kernel, 1, 1024, f);
+  return chain.launch("luma_grad_finish_kernel", luma_grad_finish_kernel, 1, 1024,
+                      finish_args(a, n_partials));
 }
 
 int check_norm(const char* what, const LumaGradArgs* a) {
@@ -745,31 +918,88 @@ int check_norm(const char* what, const LumaGradArgs* a) {
   return LUMA_OK;
 }
 
+// The instance of a kernel template for a norm kind.
+#define LUMA_BY_KIND(kind, K, ...)                             \
+  ((kind) == LUMA_NORM_1   ? K<LUMA_NORM_1 __VA_OPT__(,) __VA_ARGS__>   \
+   : (kind) == LUMA_NORM_2 ? K<LUMA_NORM_2 __VA_OPT__(,) __VA_ARGS__>   \
+                           : K<LUMA_NORM_MAX __VA_OPT__(,) __VA_ARGS__>)
+
+template <class T>
 int norm_of(const LumaGradArgs* a, Chain& chain) {
-  auto* kernel = a->norm_kind == LUMA_NORM_1   ? luma_grad_norm_kernel<LUMA_NORM_1>
-                 : a->norm_kind == LUMA_NORM_2 ? luma_grad_norm_kernel<LUMA_NORM_2>
-                                               : luma_grad_norm_kernel<LUMA_NORM_MAX>;
-  int64_t tiles_all = 0;
-  int s = for_tables(a, a->grads, a->dtypes, nullptr, nullptr, &tiles_all,
-                     [&](const Table& t, int64_t begin, int64_t tiles, int64_t first) {
-    int r = chain.launch("luma_grad_norm_kernel", kernel, tiles, kThreads, t,
-                         a->partials + first);
-    if (r == LUMA_OK && a->norms != nullptr)
-      r = chain.launch("luma_grad_tensor_finish_kernel", luma_grad_tensor_finish_kernel, t.n,
-                       kTensorThreads, t, a->norm_kind, a->partials + first, a->norms + begin);
-    return r;
+  const bool tensors = a->norms != nullptr;
+  const int64_t tile = tile_size(total_bytes(a), kNormTile, tensors ? LUMA_GRAD_TILES : kManyTiles);
+  auto* kernel = LUMA_BY_KIND(a->norm_kind, luma_grad_norm_kernel, T);
+  int64_t partials = 0;
+  int s = for_tables<T>(a, tile, [&](const T& t, int64_t, int64_t tiles) {
+    const int64_t grid = tensors ? tiles : chain.grid(kernel, tiles);
+    double* const to = a->partials + partials;
+    partials += grid;
+    return chain.launch("luma_grad_norm_kernel", kernel, grid, kThreads, t, to);
   });
-  if (s == LUMA_OK) s = finish(a, tiles_all, chain);
+  // behind all the norms, so that those follow one another without a gap
+  int64_t from = 0;
+  if (s == LUMA_OK && tensors)
+    s = for_tables<T>(a, tile, [&](const T& t, int64_t begin, int64_t tiles) {
+      const double* const p = a->partials + from;
+      from += tiles;
+      return chain.launch("luma_grad_tensor_finish_kernel", luma_grad_tensor_finish_kernel<T>, t.n,
+                          kTensorThreads, t, a->norm_kind, p, a->norms + begin);
+    });
+  if (s == LUMA_OK) s = finish(a, partials, chain);
   return s;
 }
 
+template <class T>
 int scale_of(const LumaGradArgs* a, float host_scale, const float* scale, Chain& chain) {
-  int64_t tiles_all = 0;
-  return for_tables(a, a->grads, a->dtypes, nullptr, nullptr, &tiles_all,
-                    [&](const Table& t, int64_t, int64_t tiles, int64_t) {
-    return chain.launch("luma_grad_scale_kernel", luma_grad_scale_kernel, tiles, kThreads, t,
+  const int64_t tile = tile_size(total_bytes(a), kScaleTile, kManyTiles);
+  auto* kernel = luma_grad_scale_kernel<T>;
+  return for_tables<T>(a, tile, [&](const T& t, int64_t, int64_t tiles) {
+    return chain.launch("luma_grad_scale_kernel", kernel, chain.grid(kernel, tiles), kThreads, t,
                         host_scale, scale);
   });
+}
+
+template <class T>
+int accumulate_of(const LumaGradArgs* a, Chain& chain) {
+  double total = 0.0;
+  for (int64_t i = 0; i < a->n; ++i) total += (double)a->numel[i];
+  const bool norm = a->norm_kind != LUMA_NORM_NONE;
+  auto* kernel = norm ? LUMA_BY_KIND(a->norm_kind, luma_grad_accumulate_kernel, T)
+                      : luma_grad_accumulate_kernel<LUMA_NORM_NONE, T>;
+  int64_t partials = 0;
+  int s = for_tables<T>(a, tile_size(total, kAccumulateTile, LUMA_GRAD_TILES),
+                        [&](const T& t, int64_t, int64_t tiles) {
+    double* const to = norm ? a->partials + partials : nullptr;
+    partials += tiles;
+    return chain.launch("luma_grad_accumulate_kernel", kernel, tiles, kThreads, t, a->host_scale,
+                        a->scale, a->overwrite, to);
+  });
+  if (s == LUMA_OK && norm) s = finish(a, partials, chain);
+  return s;
+}
+
+// Whether a call is one for luma_grad_small_kernel.
+constexpr double kSmallBytes = 1 << 18;
+bool small(const LumaGradArgs* a) {
+  return a->n <= Small::kMost && a->norms == nullptr && total_bytes(a) <= kSmallBytes;
+}
+
+int small_of(const LumaGradArgs* a, int clip, Chain& chain) {
+  auto* kernel = LUMA_BY_KIND(a->norm_kind, luma_grad_small_kernel);
+  return for_tables<Small>(a, kWarpTile, [&](const Small& t, int64_t, int64_t) {
+    return chain.launch("luma_grad_small_kernel", kernel, kClusterCtas, kClusterThreads, t,
+                        finish_args(a, 0), clip);
+  });
+}
+
+int norm_call(const LumaGradArgs* a, Chain& chain) {
+  if (a->n > 0 && small(a)) return small_of(a, 0, chain);
+  return a->n <= Small::kMost ? norm_of<Small>(a, chain) : norm_of<Big>(a, chain);
+}
+
+int scale_call(const LumaGradArgs* a, float host_scale, const float* scale, Chain& chain) {
+  return a->n <= Small::kMost ? scale_of<Small>(a, host_scale, scale, chain)
+                              : scale_of<Big>(a, host_scale, scale, chain);
 }
 
 int check_args(const char* what, const LumaGradArgs* a) {
@@ -791,8 +1021,8 @@ int luma_grad_norm(const LumaGradArgs* a, void* stream) {
   if (s != LUMA_OK) return s;
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  Chain chain{static_cast<cudaStream_t>(stream)};
-  return norm_of(a, chain);
+  Chain chain(a->device, stream);
+  return norm_call(a, chain);
 }
 
 int luma_grad_finish(const LumaGradArgs* a, void* stream) {
@@ -809,7 +1039,7 @@ int luma_grad_finish(const LumaGradArgs* a, void* stream) {
     return luma_fail(LUMA_ERR_INVALID, "luma_grad_finish: device %d", (int)a->device);
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  Chain chain{static_cast<cudaStream_t>(stream)};
+  Chain chain(a->device, stream);
   return finish(a, a->n_partials, chain);
 }
 
@@ -821,8 +1051,8 @@ int luma_grad_scale(const LumaGradArgs* a, void* stream) {
   if (s != LUMA_OK) return s;
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  Chain chain{static_cast<cudaStream_t>(stream)};
-  return scale_of(a, a->host_scale, a->scale, chain);
+  Chain chain(a->device, stream);
+  return scale_call(a, a->host_scale, a->scale, chain);
 }
 
 int luma_grad_clip(const LumaGradArgs* a, void* stream) {
@@ -836,9 +1066,10 @@ int luma_grad_clip(const LumaGradArgs* a, void* stream) {
   if (s != LUMA_OK) return s;
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  Chain chain{static_cast<cudaStream_t>(stream)};
-  s = norm_of(a, chain);
-  if (s == LUMA_OK) s = scale_of(a, 1.0f, a->coef, chain);
+  Chain chain(a->device, stream);
+  if (a->n > 0 && small(a)) return small_of(a, 1, chain);
+  s = norm_call(a, chain);
+  if (s == LUMA_OK) s = scale_call(a, 1.0f, a->coef, chain);
   return s;
 }
 
@@ -855,20 +1086,9 @@ int luma_grad_accumulate(const LumaGradArgs* a, void* stream) {
       return luma_fail(LUMA_ERR_INVALID, "%s: accumulator %lld is float16", what, (long long)i);
   DeviceScope dev(a->device);
   if (dev.status != LUMA_OK) return dev.status;
-  auto* kernel = a->norm_kind == LUMA_NORM_1     ? luma_grad_accumulate_kernel<LUMA_NORM_1>
-                 : a->norm_kind == LUMA_NORM_2   ? luma_grad_accumulate_kernel<LUMA_NORM_2>
-                 : a->norm_kind == LUMA_NORM_MAX ? luma_grad_accumulate_kernel<LUMA_NORM_MAX>
-                                                 : luma_grad_accumulate_kernel<LUMA_NORM_NONE>;
-  Chain chain{static_cast<cudaStream_t>(stream)};
-  int64_t tiles_all = 0;
-  s = for_tables(a, a->accs, a->acc_dtypes, a->grads, a->dtypes, &tiles_all,
-                 [&](const Table& t, int64_t, int64_t tiles, int64_t first) {
-    return chain.launch("luma_grad_accumulate_kernel", kernel, tiles, kThreads, t, a->host_scale,
-                        a->scale, a->overwrite,
-                        a->norm_kind != LUMA_NORM_NONE ? a->partials + first : nullptr);
-  });
-  if (s == LUMA_OK && a->norm_kind != LUMA_NORM_NONE) s = finish(a, tiles_all, chain);
-  return s;
+  Chain chain(a->device, stream);
+  return a->n <= SmallPair::kMost ? accumulate_of<SmallPair>(a, chain)
+                                  : accumulate_of<BigPair>(a, chain);
 }
 
 }  // extern "C"
