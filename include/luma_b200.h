@@ -392,9 +392,9 @@ int luma_mc_copy(void* mc_dst, const void* src, uint64_t bytes, void* stream);
  * norm_kind != LUMA_NORM_NONE also the results of luma_grad_norm (norms
  * excepted) for the accumulators as stored, from the same pass.
  *
- * Tensors that a call writes must not overlap one another, and a gradient may
- * share memory with an accumulator only by being it; other lists are refused
- * with LUMA_ERR_INVALID.
+ * Tensors that a call writes must not overlap one another or hold the factor
+ * `scale`, and a gradient may share memory with an accumulator only by being
+ * it; other lists are refused with LUMA_ERR_INVALID.
  */
 enum {
   LUMA_NORM_NONE = 0,

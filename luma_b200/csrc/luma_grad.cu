@@ -742,8 +742,8 @@ struct Range {
 };
 
 // Tensors a call writes must not overlap one another, nor what the call reads
-// for another element: the elements of a launch are worked on in no order.
-// src[i] may be the very elements of ptr[i].
+// for another element, the factor among it: the elements of a launch are
+// worked on in no order.  src[i] may be the very elements of ptr[i].
 int check_disjoint(const char* what, const LumaGradArgs* a, const uint64_t* ptr,
                    const uint8_t* dtype, const uint64_t* src, const uint8_t* src_dtype) {
   try {
@@ -764,11 +764,18 @@ int check_disjoint(const char* what, const LumaGradArgs* a, const uint64_t* ptr,
           return luma_fail(LUMA_ERR_INVALID, "%s: tensors %lld and %lld overlap in memory", what,
                            (long long)w[k - 1].i, (long long)w[k].i);
     }
+    if (w.empty()) return LUMA_OK;
+    const uint64_t s0 = (uint64_t)(uintptr_t)a->scale, s1 = s0 + sizeof(float);
+    for (const Range& r : w)
+      if (s0 != 0 && r.lo < s1 && s0 < r.hi)
+        return luma_fail(LUMA_ERR_INVALID, "%s: the factor lies in tensor %lld", what,
+                         (long long)r.i);
     if (src == nullptr) return LUMA_OK;
+    const uint64_t all_lo = w.front().lo, all_hi = w.back().hi;
     for (int64_t i = 0; i < a->n; ++i) {
       if (a->numel[i] == 0) continue;
       const uint64_t lo = src[i], hi = lo + (uint64_t)a->numel[i] * elem_size(src_dtype[i]);
-      if (lo == ptr[i] && src_dtype[i] == dtype[i]) continue;
+      if (hi <= all_lo || lo >= all_hi || (lo == ptr[i] && src_dtype[i] == dtype[i])) continue;
       // the first written range that ends behind lo
       size_t x = 0, y = w.size();
       while (x < y) {

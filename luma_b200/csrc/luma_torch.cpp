@@ -387,19 +387,21 @@ PyObject* py_accumulate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (s.device != d.device) raise(PyExc_ValueError, "acc and grads must be on one device");
   for (int64_t i = 0; i < d.n(); ++i) {
     const at::Tensor &x = *d.t[i], &y = *s.t[i];
-    const std::string at_i = "[" + std::to_string(i) + "]";
     if (d.code[i] == LUMA_F16)
       raise(PyExc_ValueError, "acc must be float32 or bfloat16 tensors (got float16)");
-    if (x.sizes() != y.sizes())
-      raise(PyExc_ValueError, "acc" + at_i + " and grads" + at_i + " differ in shape (got " +
-                                  shape_text(x.sizes()) + " and " + shape_text(y.sizes()) + ")");
-    if (!(x.is_contiguous() && y.is_contiguous()) && x.strides() != y.strides())
-      raise(PyExc_ValueError, "acc" + at_i + " and grads" + at_i +
-                                  " differ in the order of their dimensions in memory (strides " +
+    const bool shapes = x.sizes() == y.sizes();
+    const bool orders = (x.is_contiguous() && y.is_contiguous()) || x.strides() == y.strides();
+    if (shapes && orders && x.is_neg() == y.is_neg()) continue;
+    const std::string at_i = "[" + std::to_string(i) + "]";
+    const std::string both = "acc" + at_i + " and grads" + at_i;
+    if (!shapes)
+      raise(PyExc_ValueError, both + " differ in shape (got " + shape_text(x.sizes()) + " and " +
+                                  shape_text(y.sizes()) + ")");
+    if (!orders)
+      raise(PyExc_ValueError, both + " differ in the order of their dimensions in memory (strides " +
                                   shape_text(x.strides()) + " and " + shape_text(y.strides()) +
                                   ")");
-    if (x.is_neg() != y.is_neg())
-      raise(PyExc_ValueError, "acc" + at_i + " or grads" + at_i + " is a negated view");
+    raise(PyExc_ValueError, "acc" + at_i + " or grads" + at_i + " is a negated view");
   }
   at::Tensor hold, norm, coef;
   factor(args[2], d, "scale", c, hold);

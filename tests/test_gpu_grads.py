@@ -382,6 +382,10 @@ def test_refusals():
     v = torch.zeros(64, device="cuda")
     with pytest.raises(ValueError, match="overlap"):
         accumulate_grads_([v[:32]], [v[1:33]])
+    with pytest.raises(ValueError, match="factor"):
+        scale_grads_([v], v[3])
+    with pytest.raises(ValueError, match="factor"):
+        accumulate_grads_([v], [v.clone()], v[63:])
     with pytest.raises(ValueError, match="shape"):
         accumulate_grads_([v], [x])
     with pytest.raises(ValueError, match="order"):

@@ -123,6 +123,14 @@ def test_c_accumulate_refuses_overlap(grads, codes, accs, acc_codes, words):
     Call(grads, [8] * n, codes, accs, acc_codes).refused("luma_grad_accumulate", words)
 
 
+@pytest.mark.parametrize("name", ["luma_grad_scale", "luma_grad_accumulate"])
+@pytest.mark.parametrize("at", [65536, 65536 + 28, 65536 - 2])
+def test_c_refuses_a_factor_inside_what_is_written(name, at):
+    """Every CTA reads it while others write."""
+    Call([65536 if name == "luma_grad_scale" else 4096], [8], [F], [65536], [F],
+         scale=at).refused(name, "factor")
+
+
 # -- Python --------------------------------------------------------------------
 
 OPS = [lambda g: luma_b200.grad_norm(g), lambda g: luma_b200.clip_coef(g, 1.0),
