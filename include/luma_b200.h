@@ -405,7 +405,7 @@ enum {
 
 /* Doubles of workspace that a norm over n tensors needs. */
 #define LUMA_GRAD_TILES 16384
-#define LUMA_GRAD_PARTIALS(n) (LUMA_GRAD_TILES + 2 * (int64_t)(n))
+#define LUMA_GRAD_PARTIALS(n) (LUMA_GRAD_TILES + 3 * (int64_t)(n))
 
 typedef struct LumaGradArgs {
   const uint64_t* grads;      /* host [n]: device address of each tensor      */

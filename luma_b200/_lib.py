@@ -86,7 +86,7 @@ GRAD_TILES = 16384  # LUMA_GRAD_TILES
 
 def grad_partials(n: int) -> int:
     """LUMA_GRAD_PARTIALS(n)."""
-    return GRAD_TILES + 2 * n
+    return GRAD_TILES + 3 * n
 
 
 class LumaGradArgs(ctypes.Structure):

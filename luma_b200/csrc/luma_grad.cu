@@ -335,18 +335,26 @@ __device__ __forceinline__ void for_turns(const T& t, F&& fn) {
   for (uint32_t r = blockIdx.x; r < tiles; r += gridDim.x) fn(find_entry(t, r), r, r + 1);
 }
 
-// partials[CTA]: one for each CTA's share of the tiles, or where there are as
-// many CTAs as tiles one for each tile.
-template <int KIND, class T>
+// partials[CTA], or with TENSORS partials[CTA + entry] for every entry that the
+// CTA's share touches: along the tiles one or both of the two numbers grow, so
+// no two partials share a place and those of an entry lie side by side.
+template <int KIND, bool TENSORS, class T>
 __global__ void __launch_bounds__(kThreads, kNormCtas) luma_grad_norm_kernel(
     const __grid_constant__ T t, double* partials) {
   start_next();
   double acc = 0.0;
   for_share(t, blockIdx.x, gridDim.x, [&](int e, uint32_t r0, uint32_t r1) {
     acc = norm_any<KIND, kThreads>(t, e, r0, r1, threadIdx.x, acc);
+    if constexpr (TENSORS) {
+      acc = block_join(KIND, acc);
+      if (threadIdx.x == 0) partials[blockIdx.x + e] = acc;
+      acc = 0.0;
+    }
   });
-  acc = block_join(KIND, acc);
-  if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  if constexpr (!TENSORS) {
+    acc = block_join(KIND, acc);
+    if (threadIdx.x == 0) partials[blockIdx.x] = acc;
+  }
   wait_for_previous();  // the table before this one: other tensors, other partials
 }
 
@@ -369,16 +377,26 @@ __device__ __forceinline__ double join_partials(int kind, const double* partials
 
 constexpr int kTensorThreads = 128;
 
-// One CTA per tensor.
+// One CTA per tensor: its norm, and its power for the total.  `ctas` is the
+// grid that left the partials.
 template <class T>
 __global__ void __launch_bounds__(kTensorThreads) luma_grad_tensor_finish_kernel(
-    const __grid_constant__ T t, int kind, const double* partials, float* norms) {
+    const __grid_constant__ T t, int kind, uint32_t ctas, const double* partials, double* powers,
+    float* norms) {
   wait_for_previous();
   start_next();
   const int e = blockIdx.x;
-  const double acc = join_partials<kTensorThreads>(kind, partials + t.first[e],
-                                                   t.first[e + 1] - t.first[e]);
-  if (threadIdx.x == 0) norms[e] = (float)(kind == LUMA_NORM_2 ? sqrt(acc) : acc);
+  const uint64_t tiles = t.first[t.n], r0 = t.first[e], r1 = t.first[e + 1];
+  double acc = 0.0;
+  if (r0 < r1) {
+    // the CTA whose share holds tile r: the first c with r + 1 <= tiles (c + 1) / ctas
+    const uint32_t c0 = (uint32_t)(((r0 + 1) * ctas - 1) / tiles);
+    const uint32_t c1 = (uint32_t)((r1 * ctas - 1) / tiles);
+    acc = join_partials<kTensorThreads>(kind, partials + c0 + e, c1 - c0 + 1);
+  }
+  if (threadIdx.x != 0) return;
+  powers[e] = acc;
+  norms[e] = (float)(kind == LUMA_NORM_2 ? sqrt(acc) : acc);
 }
 
 // One thread's work on the joined partials; returns the coefficient.
@@ -799,8 +817,8 @@ int64_t tile_size(double total, int64_t least, int64_t most) {
   return tile;
 }
 
-// At most about LUMA_GRAD_TILES where tiles have a partial each; elsewhere
-// their number only has to stay within 32 bits.
+// Accumulation has a partial for each tile, about LUMA_GRAD_TILES at most;
+// elsewhere their number only has to stay within 32 bits.
 constexpr int64_t kManyTiles = (int64_t)1 << 30;
 
 double total_bytes(const LumaGradArgs* a) {
@@ -934,26 +952,29 @@ int check_norm(const char* what, const LumaGradArgs* a) {
 template <class T>
 int norm_of(const LumaGradArgs* a, Chain& chain) {
   const bool tensors = a->norms != nullptr;
-  const int64_t tile = tile_size(total_bytes(a), kNormTile, tensors ? LUMA_GRAD_TILES : kManyTiles);
-  auto* kernel = LUMA_BY_KIND(a->norm_kind, luma_grad_norm_kernel, T);
-  int64_t partials = 0;
+  const int64_t tile = tile_size(total_bytes(a), kNormTile, kManyTiles);
+  auto* kernel = tensors ? LUMA_BY_KIND(a->norm_kind, luma_grad_norm_kernel, true, T)
+                         : LUMA_BY_KIND(a->norm_kind, luma_grad_norm_kernel, false, T);
+  int64_t partials = tensors ? a->n : 0;  // behind the tensors' powers
   int s = for_tables<T>(a, tile, [&](const T& t, int64_t, int64_t tiles) {
-    const int64_t grid = tensors ? tiles : chain.grid(kernel, tiles);
+    const int64_t grid = chain.grid(kernel, tiles);
     double* const to = a->partials + partials;
-    partials += grid;
+    partials += grid + (tensors ? t.n : 0);
     return chain.launch("luma_grad_norm_kernel", kernel, grid, kThreads, t, to);
   });
+  if (s != LUMA_OK) return s;
+  if (!tensors) return finish(a, partials, chain);
   // behind all the norms, so that those follow one another without a gap
-  int64_t from = 0;
-  if (s == LUMA_OK && tensors)
-    s = for_tables<T>(a, tile, [&](const T& t, int64_t begin, int64_t tiles) {
-      const double* const p = a->partials + from;
-      from += tiles;
-      return chain.launch("luma_grad_tensor_finish_kernel", luma_grad_tensor_finish_kernel<T>, t.n,
-                          kTensorThreads, t, a->norm_kind, p, a->norms + begin);
-    });
-  if (s == LUMA_OK) s = finish(a, partials, chain);
-  return s;
+  partials = a->n;
+  s = for_tables<T>(a, tile, [&](const T& t, int64_t begin, int64_t tiles) {
+    const int64_t grid = chain.grid(kernel, tiles);
+    const double* const from = a->partials + partials;
+    partials += grid + t.n;
+    return chain.launch("luma_grad_tensor_finish_kernel", luma_grad_tensor_finish_kernel<T>, t.n,
+                        kTensorThreads, t, a->norm_kind, (uint32_t)grid, from,
+                        a->partials + begin, a->norms + begin);
+  });
+  return s == LUMA_OK ? finish(a, a->n, chain) : s;
 }
 
 template <class T>
@@ -986,7 +1007,7 @@ int accumulate_of(const LumaGradArgs* a, Chain& chain) {
 }
 
 // Whether a call is one for luma_grad_small_kernel.
-constexpr double kSmallBytes = 1 << 18;
+constexpr double kSmallBytes = 1 << 19;
 bool small(const LumaGradArgs* a) {
   return a->n <= Small::kMost && a->norms == nullptr && total_bytes(a) <= kSmallBytes;
 }
