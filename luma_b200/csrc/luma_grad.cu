@@ -18,6 +18,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <exception>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -764,48 +765,44 @@ struct Range {
 // worked on in no order.  src[i] may be the very elements of ptr[i].
 int check_disjoint(const char* what, const LumaGradArgs* a, const uint64_t* ptr,
                    const uint8_t* dtype, const uint64_t* src, const uint8_t* src_dtype) {
-  try {
-    std::vector<Range> w;
-    w.reserve((size_t)a->n);
-    bool sorted = true;
-    for (int64_t i = 0; i < a->n; ++i) {
-      if (a->numel[i] == 0) continue;
-      const uint64_t hi = ptr[i] + (uint64_t)a->numel[i] * elem_size(dtype[i]);
-      if (!w.empty() && ptr[i] < w.back().hi) sorted = false;
-      w.push_back({ptr[i], hi, i});
+  std::vector<Range> w;
+  w.reserve((size_t)a->n);
+  bool sorted = true;
+  for (int64_t i = 0; i < a->n; ++i) {
+    if (a->numel[i] == 0) continue;
+    const uint64_t hi = ptr[i] + (uint64_t)a->numel[i] * elem_size(dtype[i]);
+    if (!w.empty() && ptr[i] < w.back().hi) sorted = false;
+    w.push_back({ptr[i], hi, i});
+  }
+  auto by_lo = [](const Range& x, const Range& y) { return x.lo < y.lo; };
+  if (!sorted) {
+    std::sort(w.begin(), w.end(), by_lo);
+    for (size_t k = 1; k < w.size(); ++k)
+      if (w[k].lo < w[k - 1].hi)
+        return luma_fail(LUMA_ERR_INVALID, "%s: tensors %lld and %lld overlap in memory", what,
+                         (long long)w[k - 1].i, (long long)w[k].i);
+  }
+  if (w.empty()) return LUMA_OK;
+  const uint64_t s0 = (uint64_t)(uintptr_t)a->scale, s1 = s0 + sizeof(float);
+  for (const Range& r : w)
+    if (s0 != 0 && r.lo < s1 && s0 < r.hi)
+      return luma_fail(LUMA_ERR_INVALID, "%s: the factor lies in tensor %lld", what,
+                       (long long)r.i);
+  if (src == nullptr) return LUMA_OK;
+  const uint64_t all_lo = w.front().lo, all_hi = w.back().hi;
+  for (int64_t i = 0; i < a->n; ++i) {
+    if (a->numel[i] == 0) continue;
+    const uint64_t lo = src[i], hi = lo + (uint64_t)a->numel[i] * elem_size(src_dtype[i]);
+    if (hi <= all_lo || lo >= all_hi || (lo == ptr[i] && src_dtype[i] == dtype[i])) continue;
+    // the first written range that ends behind lo
+    size_t x = 0, y = w.size();
+    while (x < y) {
+      const size_t m = (x + y) / 2;
+      if (w[m].hi > lo) y = m; else x = m + 1;
     }
-    auto by_lo = [](const Range& x, const Range& y) { return x.lo < y.lo; };
-    if (!sorted) {
-      std::sort(w.begin(), w.end(), by_lo);
-      for (size_t k = 1; k < w.size(); ++k)
-        if (w[k].lo < w[k - 1].hi)
-          return luma_fail(LUMA_ERR_INVALID, "%s: tensors %lld and %lld overlap in memory", what,
-                           (long long)w[k - 1].i, (long long)w[k].i);
-    }
-    if (w.empty()) return LUMA_OK;
-    const uint64_t s0 = (uint64_t)(uintptr_t)a->scale, s1 = s0 + sizeof(float);
-    for (const Range& r : w)
-      if (s0 != 0 && r.lo < s1 && s0 < r.hi)
-        return luma_fail(LUMA_ERR_INVALID, "%s: the factor lies in tensor %lld", what,
-                         (long long)r.i);
-    if (src == nullptr) return LUMA_OK;
-    const uint64_t all_lo = w.front().lo, all_hi = w.back().hi;
-    for (int64_t i = 0; i < a->n; ++i) {
-      if (a->numel[i] == 0) continue;
-      const uint64_t lo = src[i], hi = lo + (uint64_t)a->numel[i] * elem_size(src_dtype[i]);
-      if (hi <= all_lo || lo >= all_hi || (lo == ptr[i] && src_dtype[i] == dtype[i])) continue;
-      // the first written range that ends behind lo
-      size_t x = 0, y = w.size();
-      while (x < y) {
-        const size_t m = (x + y) / 2;
-        if (w[m].hi > lo) y = m; else x = m + 1;
-      }
-      if (x < w.size() && w[x].lo < hi)
-        return luma_fail(LUMA_ERR_INVALID, "%s: gradient %lld overlaps accumulator %lld in memory",
-                         what, (long long)i, (long long)w[x].i);
-    }
-  } catch (const std::bad_alloc&) {
-    return luma_fail(LUMA_ERR_INVALID, "%s: out of host memory", what);
+    if (x < w.size() && w[x].lo < hi)
+      return luma_fail(LUMA_ERR_INVALID, "%s: gradient %lld overlaps accumulator %lld in memory",
+                       what, (long long)i, (long long)w[x].i);
   }
   return LUMA_OK;
 }
@@ -917,7 +914,9 @@ struct Chain {
     cfg.numAttrs = first ? 0 : 1;
     first = false;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
-    return e == cudaSuccess ? LUMA_OK : luma_cuda_fail(e, what);
+    if (e == cudaSuccess) return LUMA_OK;
+    cudaGetLastError();  // reported here, not by a later call
+    return luma_cuda_fail(e, what);
   }
 };
 
@@ -1038,12 +1037,7 @@ int check_args(const char* what, const LumaGradArgs* a) {
   return check_list(what, a->grads, a->dtypes, a->numel, a->n);
 }
 
-}  // namespace
-
-extern "C" {
-
-int luma_grad_norm(const LumaGradArgs* a, void* stream) {
-  luma_g_err[0] = '\0';
+int grad_norm(const LumaGradArgs* a, void* stream) {
   int s = check_args("luma_grad_norm", a);
   if (s == LUMA_OK) s = check_norm("luma_grad_norm", a);
   if (s != LUMA_OK) return s;
@@ -1053,8 +1047,7 @@ int luma_grad_norm(const LumaGradArgs* a, void* stream) {
   return norm_call(a, chain);
 }
 
-int luma_grad_finish(const LumaGradArgs* a, void* stream) {
-  luma_g_err[0] = '\0';
+int grad_finish(const LumaGradArgs* a, void* stream) {
   if (a == nullptr) return luma_fail(LUMA_ERR_INVALID, "luma_grad_finish: NULL args");
   if (a->partials == nullptr || a->n_partials < 0)
     return luma_fail(LUMA_ERR_INVALID, "luma_grad_finish: no partials");
@@ -1071,8 +1064,7 @@ int luma_grad_finish(const LumaGradArgs* a, void* stream) {
   return finish(a, a->n_partials, chain);
 }
 
-int luma_grad_scale(const LumaGradArgs* a, void* stream) {
-  luma_g_err[0] = '\0';
+int grad_scale(const LumaGradArgs* a, void* stream) {
   int s = check_args("luma_grad_scale", a);
   if (s == LUMA_OK)
     s = check_disjoint("luma_grad_scale", a, a->grads, a->dtypes, nullptr, nullptr);
@@ -1083,8 +1075,7 @@ int luma_grad_scale(const LumaGradArgs* a, void* stream) {
   return scale_call(a, a->host_scale, a->scale, chain);
 }
 
-int luma_grad_clip(const LumaGradArgs* a, void* stream) {
-  luma_g_err[0] = '\0';
+int grad_clip(const LumaGradArgs* a, void* stream) {
   int s = check_args("luma_grad_clip", a);
   if (s == LUMA_OK) s = check_norm("luma_grad_clip", a);
   if (s == LUMA_OK && a->coef == nullptr)
@@ -1101,8 +1092,7 @@ int luma_grad_clip(const LumaGradArgs* a, void* stream) {
   return s;
 }
 
-int luma_grad_accumulate(const LumaGradArgs* a, void* stream) {
-  luma_g_err[0] = '\0';
+int grad_accumulate(const LumaGradArgs* a, void* stream) {
   const char* what = "luma_grad_accumulate";
   int s = check_args(what, a);
   if (s == LUMA_OK) s = check_list(what, a->accs, a->acc_dtypes, a->numel, a->n);
@@ -1117,6 +1107,41 @@ int luma_grad_accumulate(const LumaGradArgs* a, void* stream) {
   Chain chain(a->device, stream);
   return a->n <= SmallPair::kMost ? accumulate_of<SmallPair>(a, chain)
                                   : accumulate_of<BigPair>(a, chain);
+}
+
+// No exception leaves a C entry.
+int guarded(const char* what, int (*fn)(const LumaGradArgs*, void*), const LumaGradArgs* a,
+            void* stream) {
+  luma_g_err[0] = '\0';
+  try {
+    return fn(a, stream);
+  } catch (const std::exception& e) {
+    return luma_fail(LUMA_ERR_INVALID, "%s: %s", what, e.what());
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int luma_grad_norm(const LumaGradArgs* args, void* stream) {
+  return guarded("luma_grad_norm", grad_norm, args, stream);
+}
+
+int luma_grad_finish(const LumaGradArgs* args, void* stream) {
+  return guarded("luma_grad_finish", grad_finish, args, stream);
+}
+
+int luma_grad_scale(const LumaGradArgs* args, void* stream) {
+  return guarded("luma_grad_scale", grad_scale, args, stream);
+}
+
+int luma_grad_clip(const LumaGradArgs* args, void* stream) {
+  return guarded("luma_grad_clip", grad_clip, args, stream);
+}
+
+int luma_grad_accumulate(const LumaGradArgs* args, void* stream) {
+  return guarded("luma_grad_accumulate", grad_accumulate, args, stream);
 }
 
 }  // extern "C"

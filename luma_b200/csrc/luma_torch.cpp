@@ -12,6 +12,8 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -296,13 +298,15 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // The sum of powers (or the maximum) of a rank's shards, one float64 on their
-// device; None where the list is empty.
+// device; 0 on the current device where the list is empty.
 PyObject* py_power(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arity("power", n, 2);  // grads, kind
   List l;
   collect(l, args[0], "grads", false);
-  if (l.n() == 0) Py_RETURN_NONE;
+  if (l.n() == 0)
+    return THPVariable_Wrap(at::zeros({1}, at::TensorOptions().dtype(at::kDouble).device(
+        c10::Device(c10::kCUDA, c10::cuda::current_device()))));
   Call c;
   set_list(c, l);
   c.a.norm_kind = (int32_t)PyLong_AsLong(args[1]);

@@ -74,9 +74,7 @@ def _check_finite(norm: torch.Tensor) -> None:
 def _over_ranks(grads, kind: int, group, max_norm=None, inv_scale=None, found_inf=None):
     """(norm, coef or None) of the lists of all ranks in `group` together."""
     import torch.distributed as dist
-    power = _ops().power(grads, kind)
-    if power is None:  # a rank without shards adds nothing
-        power = torch.zeros(1, dtype=torch.float64, device="cuda")
+    power = _ops().power(grads, kind)  # 0 of a rank without shards
     if kind == _lib.NORM_MAX:
         # a maximum over ranks may drop a NaN, but no infinity
         power.nan_to_num_(nan=math.inf, posinf=math.inf)

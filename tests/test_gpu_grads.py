@@ -71,6 +71,9 @@ SIZES = {
     "one": [1], "few": [31, 33, 1, 2, 3], "empty between": [5, 0, 1024, 0, 0, 7, 0],
     "tile ends": [16383, 16384, 16385, 65536, 32768 + 1], "long": [1_000_003],
     "many": list(range(1, 300)), "more than a table": [3, 0, 17, 1] * 700, "none": [0, 0],
+    # around the ends of what one cluster takes: 128 tensors, 512 KB
+    "128 tensors": [1, 2, 40, 700] * 32, "129 tensors": [5] * 129,
+    "512 KB of fp32": [65_536, 0, 65_536], "more than 512 KB": [131_073, 131_072],
 }
 
 
@@ -461,6 +464,68 @@ def test_two_captured_graphs_replayed_at_once():
             r3, rc = accumulate_grads_(ref, ts, norm_type=1.0, max_norm=3.0)
             assert torch.equal(r3, n3) and torch.equal(rc, coef)
             assert all(torch.equal(a, b) for a, b in zip(ref, acc))
+
+
+def test_first_call_in_a_capture():
+    """A process whose first calls are captured: nothing is left to be set up
+    that a capture forbids."""
+    import subprocess
+    import sys
+    code = """
+import torch, luma_b200
+x = [torch.full((n,), 2.0, device="cuda") for n in (9, 300_000)]
+y = [torch.zeros_like(t) for t in x]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = luma_b200.accumulate_grads_(y, x, 0.5, norm_type=2.0)
+    b, c = luma_b200.grad_norm(x, per_tensor=True)
+    d = luma_b200.clip_grads_(y, 1.0)
+    e = luma_b200.clip_grads_(x[:1], 3.0)
+g.replay()
+torch.cuda.synchronize()
+assert abs(float(a) - 300_009 ** 0.5) < 1e-3 and abs(float(b) - 2 * 300_009 ** 0.5) < 1e-3
+assert float(c[0]) == 6.0 and torch.equal(a, d) and float(e) == 6.0
+assert abs(float(luma_b200.grad_norm(y)) - 1) < 1e-5 and abs(float(x[0][0]) - 1) < 1e-5
+"""
+    root = luma_b200.__path__[0].rsplit("/", 1)[0]
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
+
+
+def test_c_entries_without_torch_lists():
+    """The C ABI as another host uses it: its own arrays, a workspace of its
+    own, the power of two halves reduced by the caller."""
+    import ctypes
+    from array import array
+    from luma_b200 import _lib
+    h = _lib.lib()
+    flat, ts = make([1000, 0, 70_001, 5], BF16, offset=3)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    out = torch.full((8,), -1.0, dtype=torch.float64, device="cuda")
+    powers = torch.full((2,), -1.0, dtype=torch.float64, device="cuda")
+    for k, part in enumerate((ts[:2], ts[2:])):
+        a = _lib.LumaGradArgs()
+        ptrs = array("Q", [t.data_ptr() for t in part])
+        numels = array("q", [t.numel() for t in part])
+        codes = bytes([_lib.BF16] * len(part))
+        a.grads, a.numel = ptrs.buffer_info()[0], numels.buffer_info()[0]
+        a.dtypes = ctypes.cast(ctypes.c_char_p(codes), ctypes.c_void_p)
+        a.n, a.norm_kind = len(part), _lib.NORM_2
+        ws = torch.empty(_lib.grad_partials(len(part)), dtype=torch.float64, device="cuda")
+        a.partials, a.n_partials = ws.data_ptr(), ws.numel()
+        a.power = powers[k:].data_ptr()
+        assert h.luma_grad_norm(ctypes.byref(a), stream) == _lib.LUMA_OK, h.luma_last_error()
+    near(powers[0], exact_power(ts[0], 2.0), 20 * U)
+    a = _lib.LumaGradArgs()
+    a.partials, a.n_partials, a.norm_kind, a.max_norm = powers.data_ptr(), 2, _lib.NORM_2, 0.5
+    norm, coef = out[:1].view(torch.float32)[:1], out[1:2].view(torch.float32)[:1]
+    a.norm, a.coef = norm.data_ptr(), coef.data_ptr()
+    assert h.luma_grad_finish(ctypes.byref(a), stream) == _lib.LUMA_OK, h.luma_last_error()
+    near(norm, exact_norm(ts, 2.0), NORM_TOL[2.0])
+    near(coef, exact_coef(exact_norm(ts, 2.0), 0.5), NORM_TOL[2.0] + U)
+    assert (out[2:] == -1).all()
+    a = _lib.LumaGradArgs()  # nothing to do
+    assert h.luma_grad_scale(ctypes.byref(a), stream) == _lib.LUMA_OK
+    assert h.luma_grad_accumulate(ctypes.byref(a), stream) == _lib.LUMA_OK
 
 
 def test_compiled_callers():

@@ -206,6 +206,79 @@ def test_dense_layouts():
     assert not _dense(torch.zeros(3, 1).expand(3, 4)) and not _dense(torch.zeros(8).as_strided((4, 2), (1, 1)))
 
 
+# -- over ranks ----------------------------------------------------------------
+
+class FakeOps:
+    """The list module in elementary operations on CPU tensors."""
+
+    @staticmethod
+    def power(grads, kind):
+        x = torch.cat([torch.zeros(1, dtype=torch.float64), *(g.double().reshape(-1) for g in grads)])
+        x = x.abs()
+        return {1: x.sum(), 2: (x * x).sum(), 3: x.max()}[kind].reshape(1)
+
+    @staticmethod
+    def finish(power, kind, max_norm, inv_scale, found_inf):
+        norm = (power.sqrt() if kind == 2 else power)[0]
+        if found_inf is not None and not torch.isfinite(norm):
+            found_inf.fill_(1.0)
+        coef = None if max_norm is None else torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+        return norm, coef
+
+    @staticmethod
+    def scale(grads, coef):
+        for g in grads:
+            g.mul_(coef)
+
+
+def _rank(rank, store, ok):
+    import torch.distributed as dist
+    from luma_b200 import grads as module
+    module._ext = FakeOps
+    dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=2)
+    pg = dist.group.WORLD
+    # rank 1 holds no shards of the second list
+    mine = [torch.full((4 + rank,), 2.0 + rank)]
+    none = mine if rank == 0 else []
+    assert module.grad_norm(mine, process_group=pg) == math.sqrt(4 * 4 + 5 * 9)
+    assert module.grad_norm(mine, 1.0, process_group=pg) == 23.0
+    assert module.grad_norm(mine, math.inf, process_group=pg) == 3.0
+    assert module.grad_norm(none, process_group=pg) == 4.0
+    norm, coef = module.clip_coef(none, 2.0, process_group=pg)
+    assert norm == 4.0 and abs(coef - 0.5) < 1e-6
+    norm = module.clip_grads_(none, 2.0, process_group=pg)
+    assert norm == 4.0 and all(abs(g[0] - 1) < 1e-6 for g in none)
+    # a NaN on one rank is not lost, and raises the flag on both
+    mine[0][0] = math.nan if rank else 1.0
+    flag = torch.zeros(1)
+    norm, _ = module.clip_coef(mine, 1.0, math.inf, found_inf=flag, process_group=pg)
+    assert norm == math.inf and flag == 1.0
+    assert math.isnan(module.grad_norm(mine, process_group=pg))
+    for fn in (module.grad_norm, lambda g, **kw: module.clip_coef(g, 1.0, **kw)):
+        try:
+            fn(mine, process_group=pg, error_if_nonfinite=True)
+        except RuntimeError as e:
+            assert "not finite" in str(e)
+        else:
+            raise AssertionError("no error")
+    dist.destroy_process_group()
+    ok[rank] = 1
+
+
+def test_norm_over_two_ranks(tmp_path):
+    ctx = torch.multiprocessing.get_context("spawn")
+    ok = ctx.Array("i", 2)
+    ranks = [ctx.Process(target=_rank, args=(r, tmp_path / "store", ok)) for r in range(2)]
+    for p in ranks:
+        p.start()
+    for p in ranks:
+        p.join(120)
+        assert p.exitcode == 0
+    assert list(ok) == [1, 1]
+    with pytest.raises(ValueError, match="whole tensors"):
+        luma_b200.grad_norm([], per_tensor=True, process_group=object())
+
+
 # -- GradScaler ----------------------------------------------------------------
 
 class FakeLUMA(torch.optim.Optimizer):
