@@ -33,10 +33,15 @@ constexpr int kVec = 32;                   // bytes of the widest load
 constexpr int kBatch = 4;                  // loads in flight per thread
 constexpr int kNormBatch = 2;              // of the norm, with five CTAs on an SM
 constexpr int kNormCtas = 5;
-// tiles: one batch of a CTA
-constexpr int64_t kNormTile = (int64_t)kNormBatch * kThreads * kVec;    // bytes
-constexpr int64_t kScaleTile = (int64_t)kBatch * kThreads * kVec;       // bytes
-constexpr int64_t kAccumulateTile = (int64_t)kBatch * kThreads * 8;     // elements
+// tiles, as powers of two: one batch of a CTA, of a warp in the small kernel
+constexpr int kNormTile = 14;        // bytes
+constexpr int kScaleTile = 15;       // bytes
+constexpr int kAccumulateTile = 13;  // elements
+constexpr int kWarpTile = 11;        // bytes
+static_assert(1 << kNormTile == kNormBatch * kThreads * kVec &&
+              1 << kScaleTile == kBatch * kThreads * kVec &&
+              1 << kAccumulateTile == kBatch * kThreads * 8 &&
+              1 << kWarpTile == kNormBatch * 32 * kVec);
 
 // Tensors of one launch, at most N.  Tile t belongs to the last entry i with
 // first[i] <= t; entries without elements have no tiles.
@@ -48,10 +53,10 @@ struct Table {
   uint32_t first[N + 1];
   uint8_t dtype[N];
   int32_t n;
-  int64_t tile;            // bytes per tile
+  int32_t shift;           // a tile is 2^shift bytes
 };
 
-// The same with the gradients that are added to ptr; tiles are in elements.
+// The same with the gradients that are added to ptr; tiles are 2^shift elements.
 template <int N>
 struct PairTable : Table<N> {
   uint64_t src[N];
@@ -251,8 +256,8 @@ template <int DT, class T>
 __device__ __forceinline__ Span span_of(const T& t, int e, uint32_t r0, uint32_t r1) {
   const uint64_t p = t.ptr[e], end = p + (uint64_t)t.numel[e] * Elem<DT>::kSize;
   const uint64_t from = p & ~(uint64_t)(kVec - 1);
-  const uint64_t lo = max(p, from + (uint64_t)(r0 - t.first[e]) * t.tile);
-  const uint64_t hi = min(end, from + (uint64_t)(r1 - t.first[e]) * t.tile);
+  const uint64_t lo = max(p, from + ((uint64_t)(r0 - t.first[e]) << t.shift));
+  const uint64_t hi = min(end, from + ((uint64_t)(r1 - t.first[e]) << t.shift));
   const uint64_t v0 = (lo + kVec - 1) & ~(uint64_t)(kVec - 1);
   const uint64_t v1 = max(v0, hi & ~(uint64_t)(kVec - 1));
   return {(char*)lo, (char*)hi, (char*)v0, (char*)v1};
@@ -483,7 +488,6 @@ __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
 // joined in a fixed order, the CTAs' through distributed shared memory.
 constexpr int kClusterCtas = 8;
 constexpr int kClusterThreads = 1024;
-constexpr int64_t kWarpTile = (int64_t)kNormBatch * 32 * kVec;  // bytes
 
 template <int KIND>
 __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kClusterThreads)
@@ -580,8 +584,8 @@ __device__ __forceinline__ double accumulate_tiles(const T& t, int e, uint32_t r
   const int64_t n = t.numel[e];
   char* const a0 = (char*)t.ptr[e];
   const char* const g0 = (const char*)t.src[e];
-  int64_t lo = (int64_t)(r0 - t.first[e]) * t.tile;
-  int64_t hi = min((int64_t)(r1 - t.first[e]) * t.tile, n);
+  int64_t lo = (int64_t)(r0 - t.first[e]) << t.shift;
+  int64_t hi = min((int64_t)(r1 - t.first[e]) << t.shift, n);
   const auto one = [&](int64_t i) {
     const float old = f.overwrite ? 0.0f : load_elem<AT>(a0 + i * kA);
     float v = f(old, load_elem<GT>(g0 + i * kG));
@@ -746,7 +750,7 @@ int check_list(const char* what, const uint64_t* ptr, const uint8_t* dtype, cons
     if (dtype[i] > LUMA_F16)
       return luma_fail(LUMA_ERR_INVALID, "%s: entry %lld has unknown type %d", what, (long long)i,
                        (int)dtype[i]);
-    if (numel[i] > 0 && (ptr[i] == 0 || ptr[i] % elem_size(dtype[i]) != 0))
+    if (numel[i] > 0 && (ptr[i] == 0 || (ptr[i] & (elem_size(dtype[i]) - 1)) != 0))
       return luma_fail(LUMA_ERR_INVALID, "%s: entry %lld has a NULL or misaligned address", what,
                        (long long)i);
     if (numel[i] > (int64_t)1 << 48)
@@ -807,11 +811,12 @@ int check_disjoint(const char* what, const LumaGradArgs* a, const uint64_t* ptr,
   return LUMA_OK;
 }
 
-// A tile's size: `least`, or more where that would give more than `most` tiles.
-int64_t tile_size(double total, int64_t least, int64_t most) {
-  int64_t tile = least;
-  while ((double)tile * (double)most < total) tile *= 2;
-  return tile;
+// A tile's size as a power of two: `least`, or more where that would give more
+// than `most` tiles.
+int tile_shift(double total, int least, int64_t most) {
+  int shift = least;
+  while (std::ldexp((double)most, shift) < total) ++shift;
+  return shift;
 }
 
 // Accumulation has a partial for each tile, about LUMA_GRAD_TILES at most;
@@ -833,7 +838,7 @@ int64_t fill(Table<N>& t, int k, const LumaGradArgs* a, int64_t i) {
   t.dtype[k] = a->dtypes[i];
   if (a->numel[i] == 0) return 0;
   const int64_t bytes = a->numel[i] * elem_size(a->dtypes[i]) + (int64_t)(a->grads[i] % kVec);
-  return (bytes + t.tile - 1) / t.tile;
+  return ((bytes - 1) >> t.shift) + 1;
 }
 
 template <int N>
@@ -843,15 +848,15 @@ int64_t fill(PairTable<N>& t, int k, const LumaGradArgs* a, int64_t i) {
   t.dtype[k] = a->acc_dtypes[i];
   t.src[k] = a->grads[i];
   t.src_dtype[k] = a->dtypes[i];
-  return (a->numel[i] + t.tile - 1) / t.tile;
+  return a->numel[i] == 0 ? 0 : ((a->numel[i] - 1) >> t.shift) + 1;
 }
 
 // Calls launch(table, index of its first tensor, its tiles) for every table of
 // the call.
 template <class T, class F>
-int for_tables(const LumaGradArgs* a, int64_t tile, F&& launch) {
+int for_tables(const LumaGradArgs* a, int shift, F&& launch) {
   static thread_local T t;
-  t.tile = tile;
+  t.shift = shift;
   for (int64_t i = 0; i < a->n;) {
     const int64_t begin = i;
     int64_t tiles = 0;
@@ -951,11 +956,11 @@ int check_norm(const char* what, const LumaGradArgs* a) {
 template <class T>
 int norm_of(const LumaGradArgs* a, Chain& chain) {
   const bool tensors = a->norms != nullptr;
-  const int64_t tile = tile_size(total_bytes(a), kNormTile, kManyTiles);
+  const int shift = tile_shift(total_bytes(a), kNormTile, kManyTiles);
   auto* kernel = tensors ? LUMA_BY_KIND(a->norm_kind, luma_grad_norm_kernel, true, T)
                          : LUMA_BY_KIND(a->norm_kind, luma_grad_norm_kernel, false, T);
   int64_t partials = tensors ? a->n : 0;  // behind the tensors' powers
-  int s = for_tables<T>(a, tile, [&](const T& t, int64_t, int64_t tiles) {
+  int s = for_tables<T>(a, shift, [&](const T& t, int64_t, int64_t tiles) {
     const int64_t grid = chain.grid(kernel, tiles);
     double* const to = a->partials + partials;
     partials += grid + (tensors ? t.n : 0);
@@ -965,7 +970,7 @@ int norm_of(const LumaGradArgs* a, Chain& chain) {
   if (!tensors) return finish(a, partials, chain);
   // behind all the norms, so that those follow one another without a gap
   partials = a->n;
-  s = for_tables<T>(a, tile, [&](const T& t, int64_t begin, int64_t tiles) {
+  s = for_tables<T>(a, shift, [&](const T& t, int64_t begin, int64_t tiles) {
     const int64_t grid = chain.grid(kernel, tiles);
     const double* const from = a->partials + partials;
     partials += grid + t.n;
@@ -978,9 +983,9 @@ int norm_of(const LumaGradArgs* a, Chain& chain) {
 
 template <class T>
 int scale_of(const LumaGradArgs* a, float host_scale, const float* scale, Chain& chain) {
-  const int64_t tile = tile_size(total_bytes(a), kScaleTile, kManyTiles);
+  const int shift = tile_shift(total_bytes(a), kScaleTile, kManyTiles);
   auto* kernel = luma_grad_scale_kernel<T>;
-  return for_tables<T>(a, tile, [&](const T& t, int64_t, int64_t tiles) {
+  return for_tables<T>(a, shift, [&](const T& t, int64_t, int64_t tiles) {
     return chain.launch("luma_grad_scale_kernel", kernel, chain.grid(kernel, tiles), kThreads, t,
                         host_scale, scale);
   });
@@ -994,7 +999,7 @@ int accumulate_of(const LumaGradArgs* a, Chain& chain) {
   auto* kernel = norm ? LUMA_BY_KIND(a->norm_kind, luma_grad_accumulate_kernel, T)
                       : luma_grad_accumulate_kernel<LUMA_NORM_NONE, T>;
   int64_t partials = 0;
-  int s = for_tables<T>(a, tile_size(total, kAccumulateTile, LUMA_GRAD_TILES),
+  int s = for_tables<T>(a, tile_shift(total, kAccumulateTile, LUMA_GRAD_TILES),
                         [&](const T& t, int64_t, int64_t tiles) {
     double* const to = norm ? a->partials + partials : nullptr;
     partials += tiles;
