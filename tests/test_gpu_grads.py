@@ -73,6 +73,7 @@ SIZES = {
     "many": list(range(1, 300)), "more than a table": [3, 0, 17, 1] * 700, "none": [0, 0],
     # around the ends of what one cluster takes: 128 tensors, 512 KB
     "128 tensors": [1, 2, 40, 700] * 32, "129 tensors": [5] * 129,
+    "uneven in a cluster": [1, 100_000, 0, 3] + [17] * 60 + [20_000, 0, 1],
     "512 KB of fp32": [65_536, 0, 65_536], "more than 512 KB": [131_073, 131_072],
 }
 
