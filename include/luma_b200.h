@@ -387,8 +387,8 @@ int luma_mc_copy(void* mc_dst, const void* src, uint64_t bytes, void* stream);
  * luma_grad_clip: luma_grad_norm, then x <- round(x * *coef) in place
  * (host_scale and scale are not used).
  *
- * luma_grad_accumulate: acc <- round(acc + c * x) (one fused multiply-add), or
- * acc <- round(c * x) with overwrite != 0; accs are float32 or bfloat16.  With
+ * luma_grad_accumulate: acc <- round(fl32(acc + fl32(c * x))), or acc <-
+ * round(fl32(c * x)) with overwrite != 0; accs are float32 or bfloat16.  With
  * norm_kind != LUMA_NORM_NONE also the results of luma_grad_norm (norms
  * excepted) for the accumulators as stored, from the same pass.
  *

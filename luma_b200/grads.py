@@ -165,8 +165,8 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, *,
 @torch.compiler.disable
 def accumulate_grads_(acc, grads, scale=1.0, *, overwrite: bool = False,
                       norm_type: float | None = None, max_norm: float | None = None):
-    """``acc[i] += scale * grads[i]`` for every i, in one launch: one fused
-    multiply-add in float32 per element, rounded to the accumulator's type.
+    """``acc[i] += scale * grads[i]`` for every i, in one launch: a float32
+    product and a float32 sum per element, rounded to the accumulator's type.
     With `overwrite` it is ``acc[i] = scale * grads[i]`` (the first
     micro-batch), whatever `acc` held.
 

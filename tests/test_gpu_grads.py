@@ -9,9 +9,11 @@ The root halves that and the result is rounded once: NORM2 = 11 u, NORM1 =
 21 u; a maximum is exact.  The coefficient c * min(1, max_norm / (r + 1e-6)) is
 taken in float64 from r before its rounding: COEF2 = NORM2, likewise.
 Scaling is one float32 product and one rounding to the type, and the plain
-form's is the same: equal bits.  acc + c * x as one fused operation is off by
-u |result|, and by the accumulator type's u again; a subnormal result by half
-the smallest number there is.
+form's is the same: equal bits.  acc + c * x rounds the product (off by
+2^-24 |c x|), the sum (2^-24 of it, itself off from the result by the former:
+2^-24 (|result| + 2^-24 |c x|)) and the value stored (the type's u of that): with
+U = 2^-24, at most U |c x| + (u + U + u U) (|result| + U |c x|); a subnormal
+value by half the smallest number there is, once for each rounding.
 """
 
 import math
@@ -292,9 +294,10 @@ def test_clip_against_what_users_call():
 
 def check_accumulated(acc, before, g, c, overwrite):
     """acc against c * g (+ before) in 64 bits, where c * g is exact."""
-    want = g.double() * c + (0.0 if overwrite else before.double())
+    product = g.double() * c
+    want = product + (0.0 if overwrite else before.double())
     u = torch.finfo(acc.dtype).eps / 2
-    tol = want.abs() * (u + U + u * U) + 2.0 ** -149
+    tol = U * product.abs() + (want.abs() + U * product.abs()) * (u + U + u * U) + 2.0 ** -149
     if acc.dtype != F32:
         tol = tol + 2.0 ** -134  # half the smallest bf16 there is
     assert bool(((acc.double() - want).abs() <= tol).all())
@@ -351,6 +354,19 @@ def test_accumulate_coefficient_types_and_layouts():
         before = t._version
         accumulate_grads_([accs[0]], [gs[0]])
     assert accs[0]._version > before
+
+
+def test_accumulate_ties():
+    """A third of a multiple of three is a short number again, and where the sum
+    lies half-way between two bfloat16 values the even one is stored."""
+    k = torch.arange(1, 128, device="cuda", dtype=torch.float32)
+    g = (3 * k).to(BF16)[(3 * k) == (3 * k).to(BF16).float()]  # 3 k that bf16 holds
+    third = g.double() / 3
+    for start in (256.0, 512.0, 1024.0):
+        acc = [torch.full(g.shape, start, dtype=BF16, device="cuda")]
+        accumulate_grads_(acc, [g], 1 / 3)
+        assert torch.equal(acc[0], (start + third).to(BF16))
+        assert ((start + third) % (start / 128) == start / 256).any()  # ties are among them
 
 
 def test_accumulate_nonfinite():
