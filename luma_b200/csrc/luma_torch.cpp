@@ -202,6 +202,15 @@ void written(const List& l) {
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
 }
 
+// A one-element tensor's address.  That of a wrapper without memory of its own
+// is 0, which the library takes for "no factor" or "no flag".
+template <class T>
+T* address(T* p, const char* name) {
+  if (p == nullptr)
+    raise(PyExc_ValueError, std::string(name) + " is a tensor without memory of its own");
+  return p;
+}
+
 float* flag(PyObject* o, const List& l, const char* name, bool write) {
   if (o == Py_None) return nullptr;
   const at::Tensor* t = THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
@@ -211,8 +220,8 @@ float* flag(PyObject* o, const List& l, const char* name, bool write) {
           std::string(name) + " must be a one-element float32 CUDA tensor");
   if (t->device() != l.device)
     raise(PyExc_ValueError, std::string(name) + " must be on the gradients' device");
-  return static_cast<float*>(write ? t->mutable_data_ptr()
-                                   : const_cast<void*>(t->const_data_ptr()));
+  return static_cast<float*>(address(write ? t->mutable_data_ptr()
+                                           : const_cast<void*>(t->const_data_ptr()), name));
 }
 
 // A factor given as a number or a one-element tensor; `hold` keeps the tensor
@@ -233,7 +242,7 @@ void factor(PyObject* o, const List& l, const char* name, Call& c, at::Tensor& h
   hold = t.detach();
   if (hold.is_neg() || hold.scalar_type() != at::kFloat || hold.device() != l.device)
     hold = hold.resolve_neg().to(at::TensorOptions().dtype(at::kFloat).device(l.device), true);
-  c.a.scale = static_cast<const float*>(hold.const_data_ptr());
+  c.a.scale = static_cast<const float*>(address(hold.const_data_ptr(), name));
 }
 
 bool truth(PyObject* o) {
@@ -264,6 +273,8 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Call c;
   set_list(c, l);
   c.a.norm_kind = (int32_t)PyLong_AsLong(args[1]);
+  c.a.inv_scale = flag(args[4], l, "inv_scale", false);
+  c.a.found_inf = flag(args[5], l, "found_inf", true);
   at::Tensor norm = scalar(l), coef, norms;
   c.a.norm = norm.mutable_data_ptr<float>();
   if (args[2] != Py_None) {
@@ -276,8 +287,6 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     norms = at::empty({l.n()}, norm.options());
     c.a.norms = norms.mutable_data_ptr<float>();
   }
-  c.a.inv_scale = flag(args[4], l, "inv_scale", false);
-  c.a.found_inf = flag(args[5], l, "found_inf", true);
   set_workspace(c, l);
   if (clip) {
     launch("luma_grad_clip", luma_grad_clip, c);

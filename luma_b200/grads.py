@@ -65,6 +65,27 @@ def _bound(max_norm) -> float:
     return m
 
 
+def local_scalar(t, name: str):
+    """What this rank reads of a one-element factor: of a replicated DTensor its
+    local copy, anything else as it is.  A part of one (sharded, or a term of a
+    sum) is refused; getting the value would take a collective."""
+    if type(t) is torch.Tensor or not hasattr(t, "_local_tensor"):
+        return t
+    if not all(p.is_replicate() for p in t.placements):
+        raise ValueError(f"{name} must be replicated where it is a DTensor (got placements "
+                         f"{t.placements}; full_tensor() gives its value)")
+    with torch.no_grad():
+        return t.to_local()
+
+
+def local_flag(t, name: str):
+    """A flag that this rank writes: no DTensor, whose other copies would not
+    hear of it."""
+    if type(t) is not torch.Tensor and hasattr(t, "_local_tensor"):
+        raise ValueError(f"{name} must not be a DTensor")
+    return t
+
+
 def _check_finite(norm: torch.Tensor) -> None:
     if not math.isfinite(float(norm)):
         raise RuntimeError("the gradients' norm is not finite, so they cannot be clipped "
@@ -122,10 +143,12 @@ def clip_coef(grads, max_norm: float, norm_type: float = 2.0, *,
     `inv_scale`, a one-element float32 CUDA tensor, is the reciprocal of the
     loss scale the grads carry: the norm is then that of the unscaled grads and
     `coef` holds both factors (unscaling and clipping).  `found_inf`, likewise
-    one element, is set to 1 if any element of the grads is inf or NaN, and
-    left alone otherwise.  `error_if_nonfinite` and `process_group` are as in
+    one element (and no DTensor), is set to 1 if any element of the grads is
+    inf or NaN, and left alone otherwise.  `error_if_nonfinite` and `process_group` are as in
     ``grad_norm``."""
     kind, bound = _kind(norm_type), _bound(max_norm)
+    inv_scale = local_scalar(inv_scale, "inv_scale")
+    found_inf = local_flag(found_inf, "found_inf")
     if process_group is not None:
         norm, coef = _over_ranks(grads, kind, process_group, bound, inv_scale, found_inf)
     else:
@@ -140,9 +163,9 @@ def clip_coef(grads, max_norm: float, norm_type: float = 2.0, *,
 def scale_grads_(grads, coef) -> None:
     """Multiply every tensor in `grads` by `coef` in place: each element becomes
     ``round_to_its_type(fl32(g) * fl32(coef))``.  `coef` is a number or a
-    one-element float32, bfloat16 or float16 tensor; where it is 1 the grads
-    are neither read nor written.  The tensors must not share memory."""
-    _ops().scale(grads, coef)
+    one-element float32, bfloat16 or float16 tensor (of a DTensor, a replicated
+    one); where it is 1 the grads are neither read nor written.  The tensors must not share memory."""
+    _ops().scale(grads, local_scalar(coef, "coef"))
 
 
 @torch.compiler.disable
@@ -183,7 +206,7 @@ def accumulate_grads_(acc, grads, scale=1.0, *, overwrite: bool = False,
     if norm_type is not None or max_norm is not None:
         kind = _kind(2.0 if norm_type is None else norm_type)
     bound = None if max_norm is None else _bound(max_norm)
-    out = _ops().accumulate(acc, grads, scale, overwrite, kind, bound)
+    out = _ops().accumulate(acc, grads, local_scalar(scale, "scale"), overwrite, kind, bound)
     if kind == _lib.NORM_NONE:
         return None
     norm, coef = out or (torch.tensor(0.0), torch.tensor(1.0))

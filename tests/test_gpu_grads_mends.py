@@ -1,0 +1,77 @@
+"""Gradient operators on the GPU with DTensors, host factors and views: the
+calls whose answer depends on what a tensor object is, besides its elements.
+Values are small integers and powers of two, so results are exact."""
+
+import math
+
+import pytest
+import torch
+
+import luma_b200
+from luma_b200 import LUMA, accumulate_grads_, clip_coef, clip_grads_, grad_norm, scale_grads_
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def mesh(tmp_path):
+    """The device mesh of one rank."""
+    import torch.distributed as dist
+    from torch.distributed.tensor import init_device_mesh
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        yield init_device_mesh("cuda", (1,))
+    finally:
+        dist.destroy_process_group()
+
+
+def distributed(mesh, local, kind="replicate"):
+    from torch.distributed.tensor import DTensor, Partial, Replicate, Shard
+    placement = {"replicate": Replicate(), "shard": Shard(0), "partial": Partial()}[kind]
+    return DTensor.from_local(local, mesh, [placement], run_check=False)
+
+
+def full(value, n=1):
+    return torch.full((n,), float(value), device="cuda")
+
+
+# -- factors and flags -----------------------------------------------------------
+
+def test_replicated_factors_count(mesh):
+    """A replicated DTensor is the number it holds."""
+    x, acc = full(8, 9), full(1, 9)
+    scale_grads_([x], distributed(mesh, full(0.25)))
+    assert (x == 2).all()
+    scale_grads_([x], distributed(mesh, torch.tensor(0.5, device="cuda")))
+    assert (x == 1).all()
+    accumulate_grads_([acc], [x], distributed(mesh, full(3).bfloat16()))
+    assert (acc == 4).all()
+    norm, coef = clip_coef([acc], 1e9, inv_scale=distributed(mesh, full(0.125)))
+    assert norm == 1.5 and coef == 0.125
+
+
+def test_the_coefficient_of_sharded_gradients(mesh):
+    """clip_grad_coef of DTensor gradients gives a DTensor; scaling by it clips."""
+    ps = []
+    for k in range(2):
+        p = torch.nn.Parameter(distributed(mesh, full(0, 8), "shard"))
+        p.grad = distributed(mesh, full(3 + k, 8), "shard")
+        ps.append(p)
+    norm, coef = luma_b200.clip_grad_coef(ps, 1.0)
+    scale_grads_([p.grad for p in ps], coef)
+    after = math.sqrt(sum(float(p.grad.to_local().double().square().sum()) for p in ps))
+    assert abs(after - 1) < 1e-6  # a coefficient within 4 roundings, a product within one
+
+
+@pytest.mark.parametrize("kind", ["shard", "partial"])
+def test_parts_of_a_factor_are_refused(mesh, kind):
+    x = full(8, 9)
+    part = distributed(mesh, full(0.25), kind)
+    for call in (lambda: scale_grads_([x], part), lambda: accumulate_grads_([x], [x], part),
+                 lambda: clip_coef([x], 1.0, inv_scale=part),
+                 lambda: clip_coef([x], 1.0, found_inf=part)):
+        with pytest.raises(ValueError, match="replicated|DTensor"):
+            call()
+    with pytest.raises(ValueError, match="found_inf .*DTensor"):
+        clip_coef([x], 1.0, found_inf=distributed(mesh, full(0)))
+    assert (x == 8).all()
