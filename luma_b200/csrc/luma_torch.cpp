@@ -307,7 +307,8 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // The sum of powers (or the maximum) of a rank's shards, one float64 on their
-// device; 0 on the current device where the list is empty.
+// device; 0 on the current device where the list is empty.  None where there
+// are DTensors: which ranks count them is the caller's to say.
 PyObject* py_power(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arity("power", n, 2);  // grads, kind
@@ -316,6 +317,7 @@ PyObject* py_power(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (l.n() == 0)
     return THPVariable_Wrap(at::zeros({1}, at::TensorOptions().dtype(at::kDouble).device(
         c10::Device(c10::kCUDA, c10::cuda::current_device()))));
+  if (l.sharded) Py_RETURN_NONE;
   Call c;
   set_list(c, l);
   c.a.norm_kind = (int32_t)PyLong_AsLong(args[1]);

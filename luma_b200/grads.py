@@ -92,10 +92,44 @@ def _check_finite(norm: torch.Tensor) -> None:
                            "(error_if_nonfinite=False clips them all the same)")
 
 
+def _counted(grads, group) -> list[torch.Tensor]:
+    """What this rank adds to the norm over the ranks of `group`: its part of
+    every tensor, but of a DTensor that several of them hold a copy of only
+    where it is the first of them."""
+    import torch.distributed as dist
+    rank, ranks = dist.get_rank(), set(dist.get_process_group_ranks(group))
+    known = {}  # (mesh, placements) -> whether this rank counts
+
+    def counts(mesh, placements):
+        if any(p.is_partial() for p in placements):
+            raise ValueError("a DTensor with Partial placement holds terms of a sum, which have no "
+                             f"norm of the sum (got placements {placements}; redistribute it first)")
+        at = mesh.get_coordinate()
+        if at is None:  # not of this mesh: no part of the tensor
+            return False
+        copies = mesh.mesh[tuple(slice(None) if p.is_replicate() else k
+                                 for p, k in zip(placements, at))]
+        return rank == min(ranks.intersection(copies.reshape(-1).tolist()), default=rank)
+
+    out = []
+    for g in [grads] if isinstance(grads, torch.Tensor) else grads:
+        if hasattr(g, "_local_tensor"):
+            key = g.device_mesh, g.placements
+            if key not in known:
+                known[key] = counts(*key)
+            g = g._local_tensor if known[key] else g._local_tensor.new_empty(0)
+        out.append(g)
+    return out
+
+
 def _over_ranks(grads, kind: int, group, max_norm=None, inv_scale=None, found_inf=None):
     """(norm, coef or None) of the lists of all ranks in `group` together."""
     import torch.distributed as dist
+    if not isinstance(grads, (torch.Tensor, list, tuple)):
+        grads = list(grads)
     power = _ops().power(grads, kind)  # 0 of a rank without shards
+    if power is None:  # there are DTensors: which of them count takes the group
+        power = _ops().power(_counted(grads, group), kind)
     if kind == _lib.NORM_MAX:
         # a maximum over ranks may drop a NaN, but no infinity
         power.nan_to_num_(nan=math.inf, posinf=math.inf)
@@ -114,10 +148,14 @@ def grad_norm(grads, norm_type: float = 2.0, *, per_tensor: bool = False,
     ``per_tensor=True`` returns ``(norm, norms)`` with ``norms[i]`` the norm of
     ``grads[i]`` (0 for an empty one), from the same pass.  With
     ``error_if_nonfinite`` the norm is read back and an inf or NaN raises.
-    With `process_group` every rank passes shards of its own (DTensors, ZeRO
-    segments) and gets the norm over all ranks' shards; every rank of the group
-    has to call, one with an empty list included.  (There a NaN on some rank
-    gives an inf norm where `norm_type` is inf.)"""
+    With `process_group` every rank passes its own part of the gradients and
+    gets the norm over the parts of all ranks in the group; every rank of the
+    group has to call, one with an empty list included.  A DTensor that several
+    of them hold a copy of counts once, and one with a Partial placement is
+    refused.  Other tensors (ZeRO segments) count on every rank that passes
+    them: a gradient whose copies lie in plain tensors belongs into the list of
+    one rank only.  (Over ranks a NaN gives an inf norm where `norm_type` is
+    inf.)"""
     kind = _kind(norm_type)
     if process_group is not None:
         if per_tensor:

@@ -75,3 +75,32 @@ def test_parts_of_a_factor_are_refused(mesh, kind):
     with pytest.raises(ValueError, match="found_inf .*DTensor"):
         clip_coef([x], 1.0, found_inf=distributed(mesh, full(0)))
     assert (x == 8).all()
+
+
+# -- lists of DTensors --------------------------------------------------------------
+
+def test_norms_of_dtensors(mesh):
+    import torch.distributed as dist
+    world = dist.group.WORLD
+    a, b = full(3, 9), full(2, 1000)
+    for kinds in (("shard", "shard"), ("replicate", "shard"), ("replicate", "replicate")):
+        ts = [distributed(mesh, t, k) for t, k in zip((a, b), kinds)]
+        ts.append(full(6, 1))
+        assert grad_norm(ts, process_group=world) == math.sqrt(81 + 4000 + 36)
+        assert grad_norm(ts, math.inf, process_group=world) == 6.0
+        norm, coef = clip_coef(ts, 1e9, process_group=world)
+        assert norm == math.sqrt(81 + 4000 + 36) and coef == 1.0
+        with pytest.raises(ValueError, match="process_group"):
+            grad_norm(ts)
+        with pytest.raises(ValueError, match="process_group"):
+            clip_grads_(ts, 1.0)
+    assert grad_norm(distributed(mesh, a), process_group=world) == 9.0
+    ts = [distributed(mesh, a), distributed(mesh, b, "partial")]
+    for call in (grad_norm, lambda g, **kw: clip_grads_(g, 1.0, **kw)):
+        with pytest.raises(ValueError, match="Partial"):
+            call(ts, process_group=world)
+    assert (a == 3).all() and (b == 2).all()
+    ts = [distributed(mesh, full(3, 16), "shard"), distributed(mesh, full(4, 16))]
+    assert clip_grads_(ts, 10.0, process_group=world) == 20.0
+    for t, want in zip(ts, (1.5, 2.0)):
+        assert (t.to_local() / want - 1).abs().max() < 1e-6  # max_norm / (norm + 1e-6)

@@ -85,3 +85,98 @@ def test_a_scalar_without_memory_is_refused(name, call):
     """Its address is 0, which a kernel takes for "no factor"."""
     with pytest.raises(ValueError, match=f"{name} .*memory"):
         call([OnCuda()], OnCuda((1,)))
+
+
+# -- the norm over ranks -----------------------------------------------------------
+
+class Ops:
+    """The list module in elementary operations on CPU tensors; DTensors are
+    left to the caller, who knows the ranks."""
+
+    @staticmethod
+    def power(grads, kind):
+        if any(hasattr(g, "_local_tensor") for g in grads):
+            return None
+        x = torch.cat([torch.zeros(1, dtype=torch.float64), *(g.double().reshape(-1) for g in grads)])
+        x = x.abs()
+        return {1: x.sum(), 2: (x * x).sum(), 3: x.max()}[kind].reshape(1)
+
+    @staticmethod
+    def finish(power, kind, max_norm, inv_scale, found_inf):
+        norm = (power.sqrt() if kind == 2 else power)[0]
+        return norm, None if max_norm is None else torch.clamp(max_norm / (norm + 1e-6), max=1.0)
+
+    @staticmethod
+    def scale(grads, coef):
+        for g in grads:
+            g.to_local().mul_(coef)
+
+
+def _rank(rank, store, ok):
+    import torch.distributed as dist
+    from torch.distributed.tensor import DTensor, Partial, Replicate, Shard, init_device_mesh
+    from luma_b200 import grads as module
+    module._ext = Ops
+    dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=4)
+    world = dist.group.WORLD
+    mesh = init_device_mesh("cpu", (2, 2), mesh_dim_names=("copies", "shards"))
+    row, col = mesh.get_coordinate()
+
+    def tensor(value, *placements):
+        return DTensor.from_local(torch.full((3,), float(value)), mesh, placements, run_check=False)
+
+    both = tensor(2, Replicate(), Replicate())           # 3 elements of 2
+    hybrid = tensor(3 + col, Replicate(), Shard(0))      # 3 of 3, 3 of 4
+    split = tensor(1 + rank, Shard(0), Shard(0))         # 3 each of 1, 2, 3, 4
+    plain = torch.full((2,), 10.0 * rank)                # 2 each of 0, 10, 20, 30
+    everything = [both, hybrid, split, plain]
+    powers = [3 * 4, 3 * (9 + 16), 3 * (1 + 4 + 9 + 16), 2 * (100 + 400 + 900)]
+    for k in range(4):
+        assert module.grad_norm([everything[k]], process_group=world) == math.sqrt(powers[k]), k
+    assert module.grad_norm(both, process_group=world) == math.sqrt(12)
+    assert module.grad_norm(iter(everything), process_group=world) == math.sqrt(sum(powers))
+    assert module.grad_norm([both, hybrid], 1.0, process_group=world) == 6 + 21
+    assert module.grad_norm([both, hybrid], math.inf, process_group=world) == 4.0
+    norm, coef = module.clip_coef([hybrid], 1.0, process_group=world)
+    assert norm == math.sqrt(75) and abs(coef * math.sqrt(75) - 1) < 1e-5
+    # the ranks of one copy: a copy of everything
+    copy = mesh["shards"].get_group()
+    assert module.grad_norm([both, hybrid], process_group=copy) == math.sqrt(12 + 75)
+    # the two copies of one shard: counted once
+    assert module.grad_norm([hybrid], process_group=mesh["copies"].get_group()) == \
+        math.sqrt(3 * (3 + col) ** 2)
+    # clipping scales every copy
+    norm = module.clip_grads_([both, hybrid], math.sqrt(87) / 2, process_group=world)
+    assert norm == math.sqrt(87)
+    assert (both.to_local() - 1).abs().max() < 1e-6
+    assert (hybrid.to_local() - (3 + col) / 2).abs().max() < 1e-6
+    # parts of a sum have no norm of their own
+    for call in (module.grad_norm, lambda g, **kw: module.clip_coef(g, 1.0, **kw),
+                 lambda g, **kw: module.clip_grads_(g, 1.0, **kw)):
+        try:
+            call([both, tensor(1, Shard(0), Partial())], process_group=world)
+        except ValueError as e:
+            assert "Partial" in str(e)
+        else:
+            raise AssertionError("no error")
+    dist.destroy_process_group()
+    ok[rank] = 1
+
+
+def test_copies_of_a_gradient_count_once(tmp_path):
+    ctx = torch.multiprocessing.get_context("spawn")
+    ok = ctx.Array("i", 4)
+    ranks = [ctx.Process(target=_rank, args=(r, tmp_path / "store", ok)) for r in range(4)]
+    for p in ranks:
+        p.start()
+    for p in ranks:
+        p.join(180)
+        assert p.exitcode == 0
+    assert list(ok) == [1] * 4
+
+
+def test_sharded_lists_need_a_group():
+    for call in (luma_b200.grad_norm, lambda g: luma_b200.clip_coef(g, 1.0),
+                 lambda g: luma_b200.clip_grads_(g, 1.0)):
+        with pytest.raises(ValueError, match="process_group"):
+            call([like_dtensor("shard")])
