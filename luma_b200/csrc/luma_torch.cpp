@@ -47,9 +47,10 @@ struct List {
   std::vector<int64_t> numel;
   std::vector<uint8_t> code;
   c10::Device device{c10::kCPU};
-  bool sharded = false;
+  std::vector<std::pair<int64_t, PyObject*>> wrapped;  // DTensors, by their place in the list
   std::vector<Ref> keep;  // the sequence, and what its items were unwrapped to
 
+  bool sharded() const { return !wrapped.empty(); }
   int64_t n() const { return (int64_t)t.size(); }
 };
 
@@ -148,7 +149,7 @@ void collect(List& l, PyObject* o, const char* name, bool written) {
         Ref local(PyObject_GetAttrString(item, "_local_tensor"));
         if (local.o == nullptr) throw python_error();
         if (!THPVariable_Check(local.o)) raise(PyExc_TypeError, "_local_tensor is not a tensor");
-        l.sharded = true;
+        l.wrapped.emplace_back((int64_t)i, item);
         item = local.o;
         l.keep.push_back(std::move(local));
       }
@@ -266,7 +267,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool clip = truth(args[6]);
   List l;
   collect(l, args[0], "grads", clip);
-  if (l.sharded)
+  if (l.sharded())
     raise(PyExc_ValueError, "the gradients are sharded (DTensor): pass process_group, over whose "
                             "ranks the norm is taken (per_tensor norms are of whole tensors)");
   if (l.n() == 0) Py_RETURN_NONE;
@@ -317,7 +318,7 @@ PyObject* py_power(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (l.n() == 0)
     return THPVariable_Wrap(at::zeros({1}, at::TensorOptions().dtype(at::kDouble).device(
         c10::Device(c10::kCUDA, c10::cuda::current_device()))));
-  if (l.sharded) Py_RETURN_NONE;
+  if (l.sharded()) Py_RETURN_NONE;
   Call c;
   set_list(c, l);
   c.a.norm_kind = (int32_t)PyLong_AsLong(args[1]);
@@ -376,6 +377,27 @@ PyObject* py_scale(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Two DTensors of an accumulation hold the same part of tensors of one shape.
+void same_part(int64_t i, PyObject* acc, PyObject* grad) {
+  const std::string at = "[" + std::to_string(i) + "]";
+  const std::string both = "acc" + at + " and grads" + at + " differ in ";
+  const at::Tensor &x = THPVariable_Unpack(acc), &y = THPVariable_Unpack(grad);
+  if (x.sizes() != y.sizes())
+    raise(PyExc_ValueError, both + "shape (got " + shape_text(x.sizes()) + " and " +
+                                shape_text(y.sizes()) + ")");
+  for (const char* name : {"device_mesh", "placements"}) {
+    Ref a(PyObject_GetAttrString(acc, name)), b(PyObject_GetAttrString(grad, name));
+    if (a.o == nullptr || b.o == nullptr) throw python_error();
+    const int same = PyObject_RichCompareBool(a.o, b.o, Py_EQ);
+    if (same < 0) throw python_error();
+    if (same) continue;
+    Ref s(PyUnicode_FromFormat("%s%s (got %S and %S)", both.c_str(), name, a.o, b.o));
+    if (s.o == nullptr) throw python_error();
+    PyErr_SetObject(PyExc_ValueError, s.o);
+    throw python_error();
+  }
+}
+
 // (norm or None, coef or None); None where the lists are empty.
 PyObject* py_accumulate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -395,11 +417,17 @@ PyObject* py_accumulate(PyObject*, PyObject* const* args, Py_ssize_t n) {
   c.a.norm_kind = (int32_t)PyLong_AsLong(args[4]);
   if (PyErr_Occurred()) throw python_error();
   const bool norms = c.a.norm_kind != LUMA_NORM_NONE;
-  if (norms && (d.sharded || s.sharded))
+  if (norms && (d.sharded() || s.sharded()))
     raise(PyExc_ValueError, "the norm of sharded accumulators (DTensor): accumulate without one, "
                             "then clip_coef(acc, ..., process_group=...)");
   if (d.n() == 0) Py_RETURN_NONE;
   if (s.device != d.device) raise(PyExc_ValueError, "acc and grads must be on one device");
+  for (auto x = d.wrapped.begin(), y = s.wrapped.begin();
+       x != d.wrapped.end() && y != s.wrapped.end();) {
+    if (x->first < y->first) ++x;
+    else if (y->first < x->first) ++y;
+    else same_part(x->first, x->second, y->second), ++x, ++y;
+  }
   for (int64_t i = 0; i < d.n(); ++i) {
     const at::Tensor &x = *d.t[i], &y = *s.t[i];
     if (d.code[i] == LUMA_F16)

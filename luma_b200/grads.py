@@ -232,7 +232,9 @@ def accumulate_grads_(acc, grads, scale=1.0, *, overwrite: bool = False,
     micro-batch), whatever `acc` held.
 
     `acc` are float32 or bfloat16 tensors, `grads` float32, bfloat16 or float16
-    ones of the same shapes and dimension order; `scale` is a number or a
+    ones of the same shapes and dimension order (a DTensor and a DTensor also of
+    the same mesh and placements; a plain tensor beside one is a buffer for this
+    rank's part of it); `scale` is a number or a
     one-element tensor as in ``scale_grads_``.  ``grads[i]`` may be ``acc[i]``
     itself; other overlaps are refused.
 

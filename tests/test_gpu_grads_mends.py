@@ -104,3 +104,19 @@ def test_norms_of_dtensors(mesh):
     assert clip_grads_(ts, 10.0, process_group=world) == 20.0
     for t, want in zip(ts, (1.5, 2.0)):
         assert (t.to_local() / want - 1).abs().max() < 1e-6  # max_norm / (norm + 1e-6)
+
+
+def test_accumulation_of_dtensors(mesh):
+    acc, g = full(1, 9), full(2, 9)
+    for kind in ("shard", "replicate", "partial"):
+        x = distributed(mesh, acc, kind)
+        accumulate_grads_([x], [distributed(mesh, g, kind)], 0.5, overwrite=kind == "partial")
+    assert (acc == 1).all()  # written in place, the last time anew
+    accumulate_grads_([acc], [distributed(mesh, g, "shard")], 0.5)  # a buffer of this rank's own
+    assert (acc == 2).all()
+    for other in ("replicate", "partial"):
+        with pytest.raises(ValueError, match="placements"):
+            accumulate_grads_([distributed(mesh, acc, "shard")], [distributed(mesh, g, other)])
+    with pytest.raises(ValueError, match="sharded"):
+        accumulate_grads_([distributed(mesh, acc)], [distributed(mesh, g)], norm_type=2.0)
+    assert (acc == 2).all()

@@ -180,3 +180,17 @@ def test_sharded_lists_need_a_group():
                  lambda g: luma_b200.clip_grads_(g, 1.0)):
         with pytest.raises(ValueError, match="process_group"):
             call([like_dtensor("shard")])
+
+
+# -- accumulation of DTensors --------------------------------------------------------
+
+@pytest.mark.parametrize("acc,grad,word", [
+    (like_dtensor("shard"), like_dtensor("replicate"), "placements"),
+    (like_dtensor("partial"), like_dtensor("replicate"), "placements"),
+    (like_dtensor("shard"), like_dtensor("shard", mesh="another"), "mesh"),
+    (like_dtensor("shard", shape=(5,)), like_dtensor("shard", shape=(6,)), "shape"),
+])
+def test_accumulate_refuses_other_placements(acc, grad, word):
+    """Parts of equal shape that are not the same part."""
+    with pytest.raises(ValueError, match=rf"acc\[1\] and grads\[1\] differ in .*{word}"):
+        luma_b200.accumulate_grads_([like_dtensor("shard"), acc], [like_dtensor("shard"), grad])
