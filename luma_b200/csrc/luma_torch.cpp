@@ -198,9 +198,13 @@ void launch(const char* name, int (*fn)(const LumaGradArgs*, void*), const Call&
 }
 
 // Tell autograd that the tensors changed, as its own in-place operations do.
+// A DTensor has a version of its own beside its local tensor's.
 void written(const List& l) {
-  for (const at::Tensor* t : l.t)
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  const auto bump = [](const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  for (const at::Tensor* t : l.t) bump(*t);
+  for (const auto& [i, wrapper] : l.wrapped) bump(THPVariable_Unpack(wrapper));
 }
 
 // A one-element tensor's address.  That of a wrapper without memory of its own

@@ -120,3 +120,11 @@ def test_accumulation_of_dtensors(mesh):
     with pytest.raises(ValueError, match="sharded"):
         accumulate_grads_([distributed(mesh, acc)], [distributed(mesh, g)], norm_type=2.0)
     assert (acc == 2).all()
+
+
+def test_written_dtensors_change_their_version(mesh):
+    """Autograd looks at the version of the tensor it saved, the DTensor."""
+    x = distributed(mesh, full(1, 9))
+    before = x._version, x.to_local()._version
+    scale_grads_([x], 0.5)
+    assert x._version > before[0] and x.to_local()._version > before[1]
