@@ -155,6 +155,17 @@ def build_desc_table_columns(cols: Columns) -> tuple[np.ndarray, int]:
     return d, int(octs.sum())
 
 
+def _address(t: torch.Tensor | None, name: str) -> int | None:
+    """Address of an optional device scalar.  A wrapper without memory of its own
+    has address 0, which the library takes for "none"."""
+    if t is None:
+        return None
+    p = t.data_ptr()
+    if p == 0:
+        raise ValueError(f"{name} is a tensor without memory of its own")
+    return p
+
+
 class DeviceEngine:
     def __init__(self, device: torch.device):
         self.device = device
@@ -292,7 +303,7 @@ class DeviceEngine:
         for i in range(3):
             a.events[i] = None if events is None else events[i]
         a.max_ctas = max_ctas
-        a.grad_scale = None if grad_scale is None else grad_scale.data_ptr()
-        a.found_inf = None if found_inf is None else found_inf.data_ptr()
+        a.grad_scale = _address(grad_scale, "grad_scale")
+        a.found_inf = _address(found_inf, "found_inf")
         _lib.check(_lib.lib().luma_step(ctypes.byref(a), ctypes.c_void_p(stream.cuda_stream)),
                    "luma_step")

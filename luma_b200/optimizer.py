@@ -25,7 +25,7 @@ from torch.optim import Optimizer
 
 from . import _lib
 from .engine import Columns, DeviceEngine, Segment
-from .grads import clip_coef
+from .grads import clip_coef, local_flag, local_scalar
 from .hostmath import SCALE_FLOOR_M, grid_record, precompute, rows_array, step_row, step_rows
 
 _BACKENDS = {"auto", "cuda", "triton"}
@@ -459,10 +459,11 @@ class LUMA(Optimizer):
         """One optimisation step for every parameter with a gradient.
 
         ``grad_scale``: optional one-element float32 / bfloat16 / float16
-        tensor c (the clip coefficient carries the grads' dtype); every grad
-        element g is then used as ``round_to_grad_dtype(fl32(g) * fl32(c))`` —
-        what ``torch._foreach_mul_(grads, c)`` would have stored — without
-        touching the grads.  With ``c`` from ``luma_b200.clip_grad_coef`` this fuses
+        tensor c (the clip coefficient carries the grads' dtype; a DTensor has
+        to be replicated); every grad element g is then used as
+        ``round_to_grad_dtype(fl32(g) * fl32(c))`` — what
+        ``torch._foreach_mul_(grads, c)`` would have stored — without touching
+        the grads.  With ``c`` from ``luma_b200.clip_grad_coef`` this fuses
         ``clip_grad_norm_``'s rescaling pass into the step (bit-identical to
         clipping first; the reference's training loop clips before every step,
         benchmarks/bench_nanogpt.py:218-225).
@@ -481,16 +482,23 @@ class LUMA(Optimizer):
         over the grads (``luma_b200.amp.scaler_step``).  Outside capturable
         mode the flag is read back once after the launch (one host sync, as
         ``GradScaler.step`` does) to keep the per-parameter ``step`` counts."""
+        grad_scale = local_scalar(grad_scale, "grad_scale")
+        found_inf = local_flag(found_inf, "found_inf")
         if grad_scale is not None:
             if not isinstance(grad_scale, torch.Tensor) or grad_scale.numel() != 1 \
                     or grad_scale.dtype not in (torch.float32, torch.bfloat16, torch.float16):
                 raise ValueError("grad_scale must be a one-element float32, bfloat16 or "
                                  "float16 tensor")
+            grad_scale = grad_scale.reshape(1)
+            if grad_scale.data_ptr() == 0:
+                raise ValueError("grad_scale is a tensor without memory of its own")
         if found_inf is not None:
             if not isinstance(found_inf, torch.Tensor) or found_inf.numel() != 1 \
                     or found_inf.dtype != torch.float32 or not found_inf.is_cuda \
                     or not found_inf.is_contiguous():
                 raise ValueError("found_inf must be a one-element contiguous float32 CUDA tensor")
+            if found_inf.data_ptr() == 0:
+                raise ValueError("found_inf is a tensor without memory of its own")
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -611,7 +619,7 @@ class LUMA(Optimizer):
         for dev, (segs, rowmap) in per_dev.items():
             gs = None
             if grad_scale is not None:
-                gs = grad_scale.reshape(1).to(device=dev, dtype=torch.float32, non_blocking=True)
+                gs = grad_scale.to(device=dev, dtype=torch.float32, non_blocking=True)
                 gs = self._keep_scale(dev, gs)
             if self.capturable:
                 self._engine(dev).step(segs, None, self._base_seed, events=self._step_events,

@@ -52,7 +52,7 @@ from dataclasses import dataclass
 import torch
 
 from .engine import DeviceEngine, Segment
-from .grads import clip_coef, grad_norm
+from .grads import clip_coef, grad_norm, local_scalar
 from .hostmath import grid_record, rows_array, step_row
 
 ALIGN = 8
@@ -606,6 +606,13 @@ class ZeroLUMA:
                     self.consumer(b, self.staging[b % n_st])
         main.wait_stream(comm)
 
+    def _scale(self, grad_scale: torch.Tensor | None) -> torch.Tensor | None:
+        """A step's factor as the kernels read it."""
+        if grad_scale is None:
+            return None
+        grad_scale = local_scalar(grad_scale, "grad_scale")
+        return grad_scale.reshape(1).to(device=self.flat.device, dtype=torch.float32)
+
     def _grad_segments(self, grad_shard: torch.Tensor) -> list[torch.Tensor]:
         """The parts of a grad shard that belong to tensors (the alignment gaps
         and the last bucket's padding hold no gradients)."""
@@ -639,8 +646,7 @@ class ZeroLUMA:
                    grad_scale: torch.Tensor | None = None) -> None:
         """Update this rank's pieces (two kernel launches per bucket, no communication)."""
         self._check(grad_shard)
-        if grad_scale is not None:
-            grad_scale = grad_scale.reshape(1).to(device=self.flat.device, dtype=torch.float32)
+        grad_scale = self._scale(grad_scale)
         self.t += 1
         rows = self._row()
         for b in range(self.layout.buckets):
@@ -686,8 +692,7 @@ class ZeroLUMA:
         `grad_scale`: optional one-element device tensor fused into the step as
         in ``LUMA.step`` (e.g. the global clip coefficient)."""
         self._check(grad_shard)
-        if grad_scale is not None:
-            grad_scale = grad_scale.reshape(1).to(device=self.flat.device, dtype=torch.float32)
+        grad_scale = self._scale(grad_scale)
         self.t += 1
         rows = self._row()
         if self.layout.world == 1:

@@ -128,3 +128,37 @@ def test_written_dtensors_change_their_version(mesh):
     before = x._version, x.to_local()._version
     scale_grads_([x], 0.5)
     assert x._version > before[0] and x.to_local()._version > before[1]
+
+
+# -- the step's own factor ------------------------------------------------------------
+
+def test_step_with_a_replicated_coefficient(mesh):
+    ps = [torch.nn.Parameter(full(1, 100)) for _ in range(2)]
+    opts = [LUMA([p], lr=0.1) for p in ps]
+    opts[1]._base_seed = opts[0]._base_seed
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for _ in range(2):
+        g = torch.randn(100, device="cuda", generator=gen)
+        for p in ps:
+            p.grad = g
+        opts[0].step(grad_scale=full(0.01))
+        opts[1].step(grad_scale=distributed(mesh, full(0.01)))
+    assert torch.equal(*ps)
+    with pytest.raises(ValueError, match="grad_scale .*replicated"):
+        opts[0].step(grad_scale=distributed(mesh, full(1), "partial"))
+    assert torch.equal(*ps)
+
+
+def test_zero_step_with_a_replicated_coefficient(mesh):
+    from luma_b200.zero import ZeroLUMA, plan_layout
+    layout = plan_layout([1000, 7], world=1, buckets=1)
+    flats = [torch.ones(layout.total, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    zs = [ZeroLUMA(f, layout, 0) for f in flats]
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for _ in range(2):
+        grad = torch.randn(layout.shard, device="cuda", generator=gen)
+        zs[0].step(grad, grad_scale=full(0.01))
+        zs[1].step(grad, grad_scale=distributed(mesh, full(0.01)))
+    assert torch.equal(*flats)
+    with pytest.raises(ValueError, match="grad_scale .*replicated"):
+        zs[1].step(grad, grad_scale=distributed(mesh, full(0.01), "shard"))

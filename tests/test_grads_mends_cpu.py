@@ -194,3 +194,23 @@ def test_accumulate_refuses_other_placements(acc, grad, word):
     """Parts of equal shape that are not the same part."""
     with pytest.raises(ValueError, match=rf"acc\[1\] and grads\[1\] differ in .*{word}"):
         luma_b200.accumulate_grads_([like_dtensor("shard"), acc], [like_dtensor("shard"), grad])
+
+
+# -- the step's own factor -----------------------------------------------------------
+
+def test_step_refuses_distributed_scalars():
+    opt = luma_b200.LUMA([torch.nn.Parameter(torch.zeros(4))])
+    for kinds in (("shard",), ("partial",)):
+        with pytest.raises(ValueError, match="grad_scale .*replicated"):
+            opt.step(grad_scale=like_dtensor(*kinds, shape=(1,), local=OnCuda((1,))))
+    with pytest.raises(ValueError, match="found_inf .*DTensor"):
+        opt.step(found_inf=like_dtensor("replicate", shape=(1,), local=OnCuda((1,))))
+
+
+def test_step_refuses_scalars_without_memory(monkeypatch):
+    monkeypatch.setattr(OnCuda, "reshape", lambda t, *shape: t)
+    monkeypatch.setattr(OnCuda, "data_ptr", lambda t: 0)
+    opt = luma_b200.LUMA([torch.nn.Parameter(torch.zeros(4))])
+    for name in ("grad_scale", "found_inf"):
+        with pytest.raises(ValueError, match=f"{name} .*memory"):
+            opt.step(**{name: OnCuda((1,))})
