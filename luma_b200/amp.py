@@ -85,8 +85,12 @@ def clip_step(scaler: torch.amp.GradScaler, optimizer, max_norm: float, norm_typ
     ``clip_coef``); returns the norm they had, inf or NaN on a step that is
     skipped.  The grads themselves keep their values.  Also takes a disabled
     scaler (clip and step) and grads the caller already unscaled; the grads
-    have to be on one device."""
+    have to be on one device.  A closure is refused: it would change the grads
+    after their norm was taken."""
     if not scaler.is_enabled():
+        if kwargs.get("closure") is not None:
+            raise RuntimeError("clip_step does not support a closure: it would change the grads "
+                               "after their norm was taken.")
         grads = [p.grad for g in optimizer.param_groups for p in g["params"] if p.grad is not None]
         norm, coef = clip_coef(grads, max_norm, norm_type)
         optimizer.step(grad_scale=coef, **kwargs)

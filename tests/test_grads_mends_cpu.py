@@ -214,3 +214,30 @@ def test_step_refuses_scalars_without_memory(monkeypatch):
     for name in ("grad_scale", "found_inf"):
         with pytest.raises(ValueError, match=f"{name} .*memory"):
             opt.step(**{name: OnCuda((1,))})
+
+
+# -- amp.clip_step -------------------------------------------------------------------
+
+class Optimizer(torch.optim.Optimizer):
+    def __init__(self, *grads):
+        ps = [torch.nn.Parameter(torch.zeros_like(g)) for g in grads]
+        for p, g in zip(ps, grads):
+            p.grad = g
+        super().__init__(ps or [torch.nn.Parameter(torch.zeros(1))], {})
+        self.calls = []
+
+    def step(self, closure=None, *, grad_scale=None, found_inf=None):
+        self.calls.append((closure, grad_scale, found_inf))
+
+
+def test_clip_step_refuses_a_closure_with_a_disabled_scaler(monkeypatch):
+    """It would run after the norm was taken: the coefficient would be that of
+    other gradients."""
+    monkeypatch.setattr(amp, "clip_coef", lambda *a, **kw: (torch.tensor(2.0), torch.tensor(0.5)))
+    off = torch.amp.GradScaler("cpu", enabled=False)
+    opt = Optimizer(torch.ones(4))
+    with pytest.raises(RuntimeError, match="[Cc]losure"):
+        amp.clip_step(off, opt, 1.0, closure=lambda: 1.0)
+    assert opt.calls == []
+    assert amp.clip_step(off, opt, 1.0, closure=None) == 2.0
+    assert opt.calls == [(None, torch.tensor(0.5), None)]
