@@ -230,7 +230,7 @@ float* flag(PyObject* o, const List& l, const char* name, bool write) {
 }
 
 // A factor given as a number or a one-element tensor; `hold` keeps the tensor
-// that the kernels read.
+// that the kernels read, where it lies on a GPU.
 void factor(PyObject* o, const List& l, const char* name, Call& c, at::Tensor& hold) {
   if (!THPVariable_Check(o)) {
     const double v = PyFloat_AsDouble(o);
@@ -244,6 +244,12 @@ void factor(PyObject* o, const List& l, const char* name, Call& c, at::Tensor& h
        t.scalar_type() != at::kHalf))
     raise(PyExc_ValueError, std::string(name) + " must be a number or a one-element float32, "
                                                 "bfloat16 or float16 tensor");
+  if (t.is_cpu()) {
+    // read now: a copy would be queued, and read what is written here meanwhile
+    // (in a captured call, before a replay)
+    c.a.host_scale = t.item<float>();
+    return;
+  }
   hold = t.detach();
   if (hold.is_neg() || hold.scalar_type() != at::kFloat || hold.device() != l.device)
     hold = hold.resolve_neg().to(at::TensorOptions().dtype(at::kFloat).device(l.device), true);

@@ -202,7 +202,8 @@ def scale_grads_(grads, coef) -> None:
     """Multiply every tensor in `grads` by `coef` in place: each element becomes
     ``round_to_its_type(fl32(g) * fl32(coef))``.  `coef` is a number or a
     one-element float32, bfloat16 or float16 tensor (of a DTensor, a replicated
-    one); where it is 1 the grads are neither read nor written.  The tensors must not share memory."""
+    one; in host memory it is read at the call, and a captured call keeps that
+    number); where it is 1 the grads are neither read nor written.  The tensors must not share memory."""
     _ops().scale(grads, local_scalar(coef, "coef"))
 
 

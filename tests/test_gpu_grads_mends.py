@@ -162,3 +162,41 @@ def test_zero_step_with_a_replicated_coefficient(mesh):
     assert torch.equal(*flats)
     with pytest.raises(ValueError, match="grad_scale .*replicated"):
         zs[1].step(grad, grad_scale=distributed(mesh, full(0.01), "shard"))
+
+
+# -- factors in host memory --------------------------------------------------------------
+
+FACTOR_CALLS = [lambda x, c: scale_grads_([x], c),
+                lambda x, c: accumulate_grads_([x], [x.clone()], c, overwrite=True)]
+
+
+@pytest.mark.parametrize("call", FACTOR_CALLS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_host_factor_is_read_at_the_call(call, dtype):
+    """Pinned or not: what is written to it afterwards, with the call still
+    queued behind other work, belongs to the next call."""
+    for pin in (True, False):
+        c = torch.full((1,), 0.5, dtype=dtype)
+        c = c.pin_memory() if pin else c
+        x = full(8, 1000)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)
+        call(x, c)
+        c.fill_(4.0)
+        torch.cuda.synchronize()
+        assert (x == 4).all()
+
+
+@pytest.mark.parametrize("pin", [True, False])
+def test_a_host_factor_in_a_capture(pin):
+    """A replay uses the number that was captured."""
+    c = torch.full((), 0.5)
+    c = c.pin_memory() if pin else c
+    x = full(64, 1000)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        scale_grads_([x], c)
+    c.fill_(100.0)
+    graph.replay()
+    graph.replay()
+    assert (x == 16).all()
