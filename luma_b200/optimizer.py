@@ -460,10 +460,11 @@ class LUMA(Optimizer):
 
         ``grad_scale``: optional one-element float32 / bfloat16 / float16
         tensor c (the clip coefficient carries the grads' dtype; a DTensor has
-        to be replicated); every grad element g is then used as
-        ``round_to_grad_dtype(fl32(g) * fl32(c))`` — what
-        ``torch._foreach_mul_(grads, c)`` would have stored — without touching
-        the grads.  With ``c`` from ``luma_b200.clip_grad_coef`` this fuses
+        to be replicated; in host memory it is read at the call, and in a
+        captured step, where it has to be pinned, by every replay); every grad
+        element g is then used as ``round_to_grad_dtype(fl32(g) * fl32(c))`` —
+        what ``torch._foreach_mul_(grads, c)`` would have stored — without
+        touching the grads.  With ``c`` from ``luma_b200.clip_grad_coef`` this fuses
         ``clip_grad_norm_``'s rescaling pass into the step (bit-identical to
         clipping first; the reference's training loop clips before every step,
         benchmarks/bench_nanogpt.py:218-225).
@@ -619,7 +620,12 @@ class LUMA(Optimizer):
         for dev, (segs, rowmap) in per_dev.items():
             gs = None
             if grad_scale is not None:
-                gs = grad_scale.to(device=dev, dtype=torch.float32, non_blocking=True)
+                if grad_scale.is_cpu and not torch.cuda.is_current_stream_capturing():
+                    # read now: a copy would be queued, and read what is written
+                    # to pinned memory meanwhile
+                    gs = torch.full((1,), grad_scale.item(), dtype=torch.float32, device=dev)
+                else:
+                    gs = grad_scale.to(device=dev, dtype=torch.float32, non_blocking=True)
                 gs = self._keep_scale(dev, gs)
             if self.capturable:
                 self._engine(dev).step(segs, None, self._base_seed, events=self._step_events,

@@ -200,3 +200,22 @@ def test_a_host_factor_in_a_capture(pin):
     graph.replay()
     graph.replay()
     assert (x == 16).all()
+
+
+def test_step_reads_a_host_scale_at_the_call():
+    ps = [torch.nn.Parameter(full(1, 100)) for _ in range(2)]
+    opts = [LUMA([p], lr=0.1) for p in ps]
+    opts[1]._base_seed = opts[0]._base_seed
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    host = torch.ones(1).pin_memory()
+    for _ in range(2):
+        g = torch.randn(100, device="cuda", generator=gen)
+        for p in ps:
+            p.grad = g
+        opts[0].step(grad_scale=full(0.01))
+        host.fill_(0.01)
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)
+        opts[1].step(grad_scale=host)
+        host.fill_(100.0)
+    assert torch.equal(*ps)
