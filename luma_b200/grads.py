@@ -21,8 +21,8 @@ Tensors are float32, bfloat16 or float16, mixed as they come, dense in memory
 size (0 included) and alignment.  Work is queued on the device's current
 stream; results are tensors on the device and the same bits on every call with
 the same tensors.  A call may be captured in a CUDA graph; replays then work
-on the captured tensors' memory.  Where a list is empty, the result is what
-nothing adds up to (norm 0, coefficient 1), on the CPU.
+on the captured tensors' memory.  Where a list is empty, the norm is 0 and the
+coefficient that of a norm of 0, on the CPU (with an `inv_scale` on its device).
 """
 
 from __future__ import annotations
@@ -84,6 +84,14 @@ def local_flag(t, name: str):
     if type(t) is not torch.Tensor and hasattr(t, "_local_tensor"):
         raise ValueError(f"{name} must not be a DTensor")
     return t
+
+
+def _coef_of_nothing(bound: float, inv_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """The coefficient where the norm is that of no elements, 0."""
+    c = min(1.0, bound / 1e-6)
+    if inv_scale is None:
+        return torch.tensor(c)
+    return inv_scale.detach().float().reshape(()).mul(c)
 
 
 def _check_finite(norm: torch.Tensor) -> None:
@@ -191,7 +199,7 @@ def clip_coef(grads, max_norm: float, norm_type: float = 2.0, *,
         norm, coef = _over_ranks(grads, kind, process_group, bound, inv_scale, found_inf)
     else:
         out = _ops().norm(grads, kind, bound, False, inv_scale, found_inf, False)
-        norm, coef, _ = out or (torch.tensor(0.0), torch.tensor(1.0), None)
+        norm, coef, _ = out or (torch.tensor(0.0), _coef_of_nothing(bound, inv_scale), None)
     if error_if_nonfinite:
         _check_finite(norm)
     return norm, coef
@@ -250,5 +258,8 @@ def accumulate_grads_(acc, grads, scale=1.0, *, overwrite: bool = False,
     out = _ops().accumulate(acc, grads, local_scalar(scale, "scale"), overwrite, kind, bound)
     if kind == _lib.NORM_NONE:
         return None
-    norm, coef = out or (torch.tensor(0.0), torch.tensor(1.0))
+    if out is None:
+        norm, coef = torch.tensor(0.0), None if bound is None else _coef_of_nothing(bound)
+    else:
+        norm, coef = out
     return norm if bound is None else (norm, coef)

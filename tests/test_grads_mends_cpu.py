@@ -241,3 +241,18 @@ def test_clip_step_refuses_a_closure_with_a_disabled_scaler(monkeypatch):
     assert opt.calls == []
     assert amp.clip_step(off, opt, 1.0, closure=None) == 2.0
     assert opt.calls == [(None, torch.tensor(0.5), None)]
+
+
+# -- empty lists -----------------------------------------------------------------------
+
+def test_coefficient_of_an_empty_list():
+    """min(1, max_norm / 1e-6), times the unscaling."""
+    inv = torch.tensor([0.125])
+    norm, coef = luma_b200.clip_coef([], 1.0, inv_scale=inv)
+    assert norm == 0.0 and coef == 0.125 and coef.shape == () and coef.dtype == torch.float32
+    inv.fill_(1.0)
+    assert coef == 0.125  # a value of its own
+    assert luma_b200.clip_coef([], 0.0)[1] == 0.0
+    assert luma_b200.clip_coef([], 2.5e-7)[1] == 0.25
+    assert luma_b200.clip_coef([], math.inf)[1] == 1.0
+    assert luma_b200.accumulate_grads_([], [], max_norm=0.0) == (0.0, 0.0)
