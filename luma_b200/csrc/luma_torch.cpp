@@ -216,8 +216,7 @@ T* address(T* p, const char* name) {
   return p;
 }
 
-float* flag(PyObject* o, const List& l, const char* name, bool write) {
-  if (o == Py_None) return nullptr;
+const at::Tensor& device_scalar(PyObject* o, const List& l, const char* name) {
   const at::Tensor* t = THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
   if (t == nullptr || t->layout() != c10::kStrided || t->numel() != 1 ||
       t->scalar_type() != at::kFloat || !t->is_cuda())
@@ -225,8 +224,24 @@ float* flag(PyObject* o, const List& l, const char* name, bool write) {
           std::string(name) + " must be a one-element float32 CUDA tensor");
   if (t->device() != l.device)
     raise(PyExc_ValueError, std::string(name) + " must be on the gradients' device");
-  return static_cast<float*>(address(write ? t->mutable_data_ptr()
-                                           : const_cast<void*>(t->const_data_ptr()), name));
+  return *t;
+}
+
+// A factor that the kernels read; `hold` keeps it.  A negated view's memory
+// holds minus its value.
+const float* reciprocal(PyObject* o, const List& l, const char* name, at::Tensor& hold) {
+  if (o == Py_None) return nullptr;
+  hold = device_scalar(o, l, name);
+  if (hold.is_neg()) hold = hold.detach().resolve_neg();
+  return static_cast<const float*>(address(hold.const_data_ptr(), name));
+}
+
+// A flag that they write.
+float* flag(PyObject* o, const List& l, const char* name) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor& t = device_scalar(o, l, name);
+  if (t.is_neg()) raise(PyExc_ValueError, std::string(name) + " must not be a negated view");
+  return static_cast<float*>(address(t.mutable_data_ptr(), name));
 }
 
 // A factor given as a number or a one-element tensor; `hold` keeps the tensor
@@ -284,8 +299,9 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Call c;
   set_list(c, l);
   c.a.norm_kind = (int32_t)PyLong_AsLong(args[1]);
-  c.a.inv_scale = flag(args[4], l, "inv_scale", false);
-  c.a.found_inf = flag(args[5], l, "found_inf", true);
+  at::Tensor hold;
+  c.a.inv_scale = reciprocal(args[4], l, "inv_scale", hold);
+  c.a.found_inf = flag(args[5], l, "found_inf");
   at::Tensor norm = scalar(l), coef, norms;
   c.a.norm = norm.mutable_data_ptr<float>();
   if (args[2] != Py_None) {
@@ -361,8 +377,9 @@ PyObject* py_finish(PyObject*, PyObject* const* args, Py_ssize_t n) {
     c.a.coef = coef.mutable_data_ptr<float>();
   }
   if (PyErr_Occurred()) throw python_error();
-  c.a.inv_scale = flag(args[3], l, "inv_scale", false);
-  c.a.found_inf = flag(args[4], l, "found_inf", true);
+  at::Tensor hold;
+  c.a.inv_scale = reciprocal(args[3], l, "inv_scale", hold);
+  c.a.found_inf = flag(args[4], l, "found_inf");
   launch("luma_grad_finish", luma_grad_finish, c);
   Ref first(THPVariable_Wrap(norm));
   Ref second(coef.defined() ? THPVariable_Wrap(coef) : Py_NewRef(Py_None));

@@ -219,3 +219,16 @@ def test_step_reads_a_host_scale_at_the_call():
         opts[1].step(grad_scale=host)
         host.fill_(100.0)
     assert torch.equal(*ps)
+
+
+# -- views -------------------------------------------------------------------------------
+
+def test_negated_views_as_scalars():
+    """A view whose memory holds minus its value."""
+    x = full(2, 16)
+    norm, coef = clip_coef([x], 1e9, inv_scale=torch._neg_view(full(-0.25)))
+    assert norm == 2.0 and coef == 0.25
+    with pytest.raises(ValueError, match="found_inf .*negated"):
+        clip_coef([x], 1.0, found_inf=torch._neg_view(full(0)))
+    scale_grads_([x], torch._neg_view(full(-0.25)))
+    assert (x == 0.5).all()
