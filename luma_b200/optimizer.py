@@ -490,13 +490,13 @@ class LUMA(Optimizer):
                     or grad_scale.dtype not in (torch.float32, torch.bfloat16, torch.float16):
                 raise ValueError("grad_scale must be a one-element float32, bfloat16 or "
                                  "float16 tensor")
-            grad_scale = grad_scale.reshape(1)
+            grad_scale = grad_scale.reshape(1).resolve_neg()
             if grad_scale.data_ptr() == 0:
                 raise ValueError("grad_scale is a tensor without memory of its own")
         if found_inf is not None:
             if not isinstance(found_inf, torch.Tensor) or found_inf.numel() != 1 \
                     or found_inf.dtype != torch.float32 or not found_inf.is_cuda \
-                    or not found_inf.is_contiguous():
+                    or not found_inf.is_contiguous() or found_inf.is_neg():
                 raise ValueError("found_inf must be a one-element contiguous float32 CUDA tensor")
             if found_inf.data_ptr() == 0:
                 raise ValueError("found_inf is a tensor without memory of its own")

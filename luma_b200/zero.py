@@ -611,7 +611,7 @@ class ZeroLUMA:
         if grad_scale is None:
             return None
         grad_scale = local_scalar(grad_scale, "grad_scale")
-        return grad_scale.reshape(1).to(device=self.flat.device, dtype=torch.float32)
+        return grad_scale.reshape(1).resolve_neg().to(device=self.flat.device, dtype=torch.float32)
 
     def _grad_segments(self, grad_shard: torch.Tensor) -> list[torch.Tensor]:
         """The parts of a grad shard that belong to tensors (the alignment gaps

@@ -232,3 +232,19 @@ def test_negated_views_as_scalars():
         clip_coef([x], 1.0, found_inf=torch._neg_view(full(0)))
     scale_grads_([x], torch._neg_view(full(-0.25)))
     assert (x == 0.5).all()
+
+
+def test_step_with_a_negated_view():
+    ps = [torch.nn.Parameter(full(1, 100)) for _ in range(2)]
+    opts = [LUMA([p], lr=0.1) for p in ps]
+    opts[1]._base_seed = opts[0]._base_seed
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    for _ in range(2):
+        g = torch.randn(100, device="cuda", generator=gen)
+        for p in ps:
+            p.grad = g
+        opts[0].step(grad_scale=full(0.01))
+        opts[1].step(grad_scale=torch._neg_view(full(-0.01)))
+    assert torch.equal(*ps)
+    with pytest.raises(ValueError, match="found_inf"):
+        opts[0].step(found_inf=torch._neg_view(full(0)))
