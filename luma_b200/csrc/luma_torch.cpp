@@ -70,6 +70,14 @@ bool dense(const at::Tensor& t) {
   return true;
 }
 
+// Whether two dense tensors of one shape have their elements in one order.  A
+// dimension of size 1 has no place in it, whatever its stride.
+bool same_order(const at::Tensor& x, const at::Tensor& y) {
+  for (int64_t k = 0; k < x.dim(); ++k)
+    if (x.size(k) != 1 && x.stride(k) != y.stride(k)) return false;
+  return true;
+}
+
 std::string shape_text(c10::IntArrayRef v) {
   std::string s = "(";
   for (size_t k = 0; k < v.size(); ++k) s += (k ? ", " : "") + std::to_string(v[k]);
@@ -460,7 +468,7 @@ PyObject* py_accumulate(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (d.code[i] == LUMA_F16)
       raise(PyExc_ValueError, "acc must be float32 or bfloat16 tensors (got float16)");
     const bool shapes = x.sizes() == y.sizes();
-    const bool orders = (x.is_contiguous() && y.is_contiguous()) || x.strides() == y.strides();
+    const bool orders = (x.is_contiguous() && y.is_contiguous()) || (shapes && same_order(x, y));
     if (shapes && orders && x.is_neg() == y.is_neg()) continue;
     const std::string at_i = "[" + std::to_string(i) + "]";
     const std::string both = "acc" + at_i + " and grads" + at_i;

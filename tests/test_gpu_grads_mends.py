@@ -248,3 +248,17 @@ def test_step_with_a_negated_view():
     assert torch.equal(*ps)
     with pytest.raises(ValueError, match="found_inf"):
         opts[0].step(found_inf=torch._neg_view(full(0)))
+
+
+def test_strides_of_single_rows():
+    """A dimension of size 1 has a stride and no place in the order."""
+    a = torch.empty_strided((4, 1, 6), (1, 1, 4), device="cuda").fill_(1.0)
+    for strides in ((1, 24, 4), (1, 4, 4), (1, 7, 4)):
+        g = torch.empty_strided((4, 1, 6), strides, dtype=torch.bfloat16, device="cuda")
+        g.copy_(torch.arange(24, device="cuda").view(4, 1, 6))
+        assert not g.is_contiguous()
+        before = a.clone()
+        accumulate_grads_([a], [g], 2.0)
+        assert torch.equal(a, before + 2 * g.float())
+    with pytest.raises(ValueError, match="order"):
+        accumulate_grads_([a], [torch.zeros(4, 1, 6, device="cuda")])
