@@ -5,7 +5,9 @@ operators) with g++ against the installed torch.
     python -m luma_b200.build [--debug]
 
 The library statically links the CUDA runtime, so it only needs the driver
-(libcuda) at run time.  The build output stays in-tree next to the package.
+(libcuda) at run time; without torch it is built alone.  The module works with
+the torch and the Python it was built for, and says so when it is imported by
+others.  The build output stays in-tree next to the package.
 """
 
 from __future__ import annotations
@@ -47,7 +49,12 @@ def build(verbose: bool = False, extra: list[str] | None = None) -> str:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
     os.replace(OUT + ".tmp", OUT)
-    build_ext(verbose)
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        print("no torch here: the library alone is built, without the module for its tensors")
+    else:
+        build_ext(verbose)
     return OUT
 
 
@@ -58,6 +65,7 @@ def build_ext(verbose: bool = False) -> str:
     libs = cpp_extension.library_paths("cuda")
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DLUMA_TORCH_VERSION="{torch.__version__}"',
            "-I", os.path.join(ROOT, "include"),
            *(f"-isystem{p}" for p in cpp_extension.include_paths("cuda")),
            f"-isystem{sysconfig.get_paths()['include']}", EXT_SOURCE, "-o", EXT_OUT + ".tmp",
@@ -71,13 +79,25 @@ def build_ext(verbose: bool = False) -> str:
     return EXT_OUT
 
 
+def _older(out: str, deps: list[str]) -> bool:
+    return not os.path.exists(out) or any(os.path.getmtime(s) > os.path.getmtime(out) for s in deps)
+
+
 def is_stale() -> bool:
-    if not os.path.exists(OUT) or not os.path.exists(EXT_OUT):
+    header = os.path.join(ROOT, "include", "luma_b200.h")
+    if _older(OUT, [*SOURCES, header, os.path.join(HERE, "csrc", "luma_internal.h")]):
         return True
-    t = min(os.path.getmtime(OUT), os.path.getmtime(EXT_OUT))
-    deps = SOURCES + [EXT_SOURCE] + [os.path.join(ROOT, "include", "luma_b200.h"),
-                      os.path.join(HERE, "csrc", "luma_internal.h")]
-    return any(os.path.getmtime(s) > t for s in deps)
+    try:
+        import torch  # noqa: F401
+    except ImportError:
+        return False  # the library is all there can be
+    if _older(EXT_OUT, [EXT_SOURCE, header]):
+        return True
+    try:
+        from luma_b200 import _grads_ext  # noqa: F401
+    except ImportError:  # built for another torch, Python or library
+        return True
+    return False
 
 
 if __name__ == "__main__":

@@ -530,7 +530,24 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_grads_ext",
 extern "C" __attribute__((visibility("default"))) PyObject* PyInit__grads_ext(void) {
   if (luma_abi_version() != LUMA_ABI_VERSION) {
     PyErr_SetString(PyExc_ImportError, "libluma_b200.so and the tensor lists' module are of "
-                                       "different builds; run python -m luma_b200.build");
+                                       "different builds");
+    return nullptr;
+  }
+  // the layout of tensors and of Python objects is compiled in
+  if ((Py_Version >> 16) != (PY_VERSION_HEX >> 16)) {
+    PyErr_Format(PyExc_ImportError, "the tensor lists' module is built for Python %d.%d",
+                 PY_MAJOR_VERSION, PY_MINOR_VERSION);
+    return nullptr;
+  }
+  Ref torch(PyImport_ImportModule("torch"));
+  if (torch.o == nullptr) return nullptr;
+  Ref version(PyObject_GetAttrString(torch.o, "__version__"));
+  if (version.o == nullptr) return nullptr;
+  const char* text = PyUnicode_AsUTF8(version.o);
+  if (text == nullptr) return nullptr;
+  if (std::string(text) != LUMA_TORCH_VERSION) {
+    PyErr_Format(PyExc_ImportError, "the tensor lists' module is built for torch %s, this is "
+                                    "torch %s", LUMA_TORCH_VERSION, text);
     return nullptr;
   }
   return PyModule_Create(&kModule);

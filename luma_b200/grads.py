@@ -46,7 +46,10 @@ def _ops():
     global _ext
     if _ext is None:
         _lib.lib()  # with its own message where the library is missing
-        from . import _grads_ext
+        try:
+            from . import _grads_ext
+        except ImportError as e:
+            raise ImportError(f"{e}; build it with `python -m luma_b200.build`") from e
         _ext = _grads_ext
     return _ext
 

@@ -256,3 +256,44 @@ def test_coefficient_of_an_empty_list():
     assert luma_b200.clip_coef([], 2.5e-7)[1] == 0.25
     assert luma_b200.clip_coef([], math.inf)[1] == 1.0
     assert luma_b200.accumulate_grads_([], [], max_norm=0.0) == (0.0, 0.0)
+
+
+# -- the module that was built for another torch ------------------------------------------
+
+def test_module_of_another_torch_is_refused():
+    import subprocess
+    import sys
+    code = """
+import torch
+torch.__version__ = "1.0.0"
+import luma_b200
+try:
+    luma_b200.grad_norm([])
+except ImportError as e:
+    assert "luma_b200.build" in str(e) and "1.0.0" in str(e), e
+else:
+    raise AssertionError("loaded")
+from luma_b200 import build
+assert build.is_stale()
+"""
+    root = luma_b200.__path__[0].rsplit("/", 1)[0]
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
+
+
+def test_library_without_torch(monkeypatch, tmp_path):
+    """A host of the C ABI alone builds the library and is told about the rest."""
+    import builtins
+    from luma_b200 import build
+    real = builtins.__import__
+
+    def none(name, *a, **kw):
+        if name == "torch" or name.startswith("torch."):
+            raise ImportError(name)
+        return real(name, *a, **kw)
+    monkeypatch.setattr(builtins, "__import__", none)
+    ran = []
+    monkeypatch.setattr(build, "OUT", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(build.subprocess, "run", lambda cmd, check: (
+        ran.append(cmd[0]), (tmp_path / "lib.so.tmp").write_bytes(b"")))
+    assert build.build() == str(tmp_path / "lib.so")
+    assert len(ran) == 1 and "nvcc" in ran[0]
