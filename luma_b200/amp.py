@@ -80,28 +80,32 @@ def scaler_step(scaler: torch.amp.GradScaler, optimizer, *args, **kwargs):
 
 
 def clip_step(scaler: torch.amp.GradScaler, optimizer, max_norm: float, norm_type: float = 2.0,
-              **kwargs) -> torch.Tensor:
+              *, process_group=None, **kwargs) -> torch.Tensor:
     """``scaler_step`` with the unscaled grads clipped to `max_norm` (their
     ``clip_coef``); returns the norm they had, inf or NaN on a step that is
     skipped.  The grads themselves keep their values.  Also takes a disabled
     scaler (clip and step) and grads the caller already unscaled; the grads
-    have to be on one device.  A closure is refused: it would change the grads
-    after their norm was taken."""
+    have to be on one device.  With sharded grads every rank of `process_group`
+    calls, and the norm and the inf/NaN flag are those of all ranks' parts (as
+    in ``clip_coef``; grads already unscaled have ``unscale_``'s flag).  A closure is refused: it would change the grads after
+    their norm was taken."""
+    over = {} if process_group is None else {"process_group": process_group}
     if not scaler.is_enabled():
         if kwargs.get("closure") is not None:
             raise RuntimeError("clip_step does not support a closure: it would change the grads "
                                "after their norm was taken.")
         grads = [p.grad for g in optimizer.param_groups for p in g["params"] if p.grad is not None]
-        norm, coef = clip_coef(grads, max_norm, norm_type)
+        norm, coef = clip_coef(grads, max_norm, norm_type, **over)
         optimizer.step(grad_scale=coef, **kwargs)
         return norm
     grads, state = _scaled_grads(scaler, optimizer, kwargs)
     if state["stage"] is OptState.UNSCALED:
-        norm, coef = clip_coef(grads, max_norm, norm_type)
+        norm, coef = clip_coef(grads, max_norm, norm_type, **over)
         scaler.step(optimizer, grad_scale=coef, **kwargs)
         return norm
     inv_scale, found_inf = _unscaling(scaler, grads)
-    norm, coef = clip_coef(grads, max_norm, norm_type, inv_scale=inv_scale, found_inf=found_inf)
+    norm, coef = clip_coef(grads, max_norm, norm_type, inv_scale=inv_scale, found_inf=found_inf,
+                           **over)
     optimizer.step(grad_scale=coef, found_inf=found_inf, **kwargs)
     state["found_inf_per_device"] = {found_inf.device: found_inf}
     state["stage"] = OptState.STEPPED

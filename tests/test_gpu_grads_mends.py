@@ -262,3 +262,32 @@ def test_strides_of_single_rows():
         assert torch.equal(a, before + 2 * g.float())
     with pytest.raises(ValueError, match="order"):
         accumulate_grads_([a], [torch.zeros(4, 1, 6, device="cuda")])
+
+
+# -- mixed precision with sharded gradients --------------------------------------------------
+
+def test_clip_step_of_dtensors(mesh):
+    """The params of a step on the same gradients in plain tensors."""
+    import torch.distributed as dist
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    init = [torch.randn(n, device="cuda", generator=gen) for n in (1000, 7)]
+    plain = [torch.nn.Parameter(t.clone()) for t in init]
+    kinds = ("shard", "replicate")
+    shards = [torch.nn.Parameter(distributed(mesh, t.clone(), k)) for t, k in zip(init, kinds)]
+    opts = [LUMA(ps, lr=1e-2) for ps in (plain, shards)]
+    opts[1]._base_seed = opts[0]._base_seed
+    scalers = [torch.amp.GradScaler("cuda", init_scale=2.0 ** 12) for _ in opts]
+    for it in range(4):
+        raw = [torch.randn(t.shape, device="cuda", generator=gen) for t in init]
+        if it == 2:
+            raw[0][5] = math.inf
+        norms = []
+        for ps, opt, scaler, over in zip((plain, shards), opts, scalers, (None, dist.group.WORLD)):
+            scale = scaler.scale(torch.ones((), device="cuda"))
+            for p, g, k in zip(ps, raw, kinds):
+                p.grad = g * scale if ps is plain else distributed(mesh, g * scale, k)
+            norms.append(luma_b200.amp.clip_step(scaler, opt, 1.0, process_group=over))
+            scaler.update()
+        assert torch.equal(*norms) and math.isfinite(norms[0]) == (it != 2)
+        assert scalers[0].get_scale() == scalers[1].get_scale()
+        assert all(torch.equal(a, b.to_local()) for a, b in zip(plain, shards)), it

@@ -297,3 +297,27 @@ def test_library_without_torch(monkeypatch, tmp_path):
         ran.append(cmd[0]), (tmp_path / "lib.so.tmp").write_bytes(b"")))
     assert build.build() == str(tmp_path / "lib.so")
     assert len(ran) == 1 and "nvcc" in ran[0]
+
+
+def test_clip_step_over_ranks(monkeypatch):
+    """Sharded gradients take the group that their norm is reduced over."""
+    seen = []
+
+    def coef(grads, max_norm, norm_type=2.0, *, inv_scale=None, found_inf=None, process_group=None):
+        seen.append((max_norm, norm_type, inv_scale, found_inf, process_group))
+        return torch.tensor(2.0), torch.tensor(0.5)
+    monkeypatch.setattr(amp, "clip_coef", coef)
+    group = object()
+    for enabled, unscaled in ((False, False), (True, False), (True, True)):
+        scaler = torch.amp.GradScaler("cpu", enabled=enabled, init_scale=4.0)
+        scaler.scale(torch.ones(()))
+        opt = Optimizer(torch.ones(4))
+        if unscaled:
+            scaler.unscale_(opt)
+        assert amp.clip_step(scaler, opt, 0.5, math.inf, process_group=group) == 2.0
+        max_norm, norm_type, inv_scale, found_inf, over = seen.pop()
+        assert (max_norm, norm_type) == (0.5, math.inf) and over is group and not seen
+        fused = enabled and not unscaled
+        assert (inv_scale is not None) == fused and (found_inf is not None) == fused
+        (_, gs, fi), = opt.calls
+        assert gs == 0.5 and fi is found_inf
