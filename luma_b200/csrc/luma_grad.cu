@@ -624,14 +624,11 @@ luma_grad_small_tensors_kernel(const __grid_constant__ Small t, const FinishArgs
 // Eight elements of consecutive memory, aligned to their size, as loaded.
 template <int DT> struct Eight { uint32_t w[DT == LUMA_F32 ? 8 : 4]; };
 
-template <int DT, bool ONCE>
+template <int DT>
 __device__ __forceinline__ Eight<DT> load8(const char* p) {
   Eight<DT> x;
   if constexpr (DT == LUMA_F32) {
-    if constexpr (ONCE) load_once(p, x.w); else load32(p, x.w);
-  } else if constexpr (ONCE) {
-    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]) : "l"(p));
+    load32(p, x.w);
   } else {
     asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(x.w[0]), "=r"(x.w[1]), "=r"(x.w[2]), "=r"(x.w[3]) : "l"(p) : "memory");
@@ -714,8 +711,8 @@ __device__ __forceinline__ double accumulate_tiles(const T& t, int e, uint32_t r
         x[u] = Eight<AT>{};
         y[u] = Eight<GT>{};
         if (j < v1) {
-          if (!f.overwrite) x[u] = load8<AT, false>(a0 + j * kA);
-          y[u] = load8<GT, false>(g0 + j * kG);
+          if (!f.overwrite) x[u] = load8<AT>(a0 + j * kA);
+          y[u] = load8<GT>(g0 + j * kG);
         }
       }
       float all[kBatch * 8];
