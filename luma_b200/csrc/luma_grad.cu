@@ -8,11 +8,14 @@
 // replays with the table it was captured with.  More tensors than a table
 // holds are worked on by several launches.  Every tensor is cut into tiles of
 // one size; which tiles a CTA works on, where its partial result goes and in
-// which order the partial results are joined follow from the sizes alone: the
-// same tensors give the same bits on every call.
+// which order the partial results are joined follow from the tensors' sizes,
+// types and alignments (tiles begin at 32-byte lines, or where eight
+// accumulators do) and from how many CTAs the device holds: the same tensors
+// give the same bits on every call.  The same values at another alignment may
+// be summed in another order.
 //
 // All of it is bound by memory: one or two operations per element against 2 to
-// 10 bytes.  Figures below are CUDA-event times on one B200 of passes captured
+// 12 bytes.  Figures below are CUDA-event times on one B200 of passes captured
 // in a graph over three sets of inputs (copy bandwidth 6.55 TB/s; pure reads
 // reach 7.4).  "Layer" is one Llama-3-8B decoder layer, 9 tensors with 218 M
 // elements in bf16.
@@ -211,7 +214,7 @@ __device__ __forceinline__ double power_of(int kind, float x) {
 }
 
 // The powers of N elements joined onto `acc`: in float32, in four chains of
-// at most 16 additions, then in float64.  A float32 sum in [2^-100, 2^126] has
+// N / 4 additions (2 to 8 in the kernels below), then in float64.  A float32 sum in [2^-100, 2^126] has
 // not overflowed, and what its squares lost below 2^-149 is less than 2^-40 of
 // it; a sum outside (all zeros excepted) is taken again in float64.  The
 // maximum is taken on the magnitudes' bits, whose order has NaN above inf.
@@ -534,9 +537,11 @@ __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
 // A small call as a whole: the norm, its results and with `clip` the scaling.
 // One cluster of eight CTAs whose warps share the tiles; the warps' sums are
 // joined in a fixed order, the CTAs' through distributed shared memory.  One
-// launch in place of two (norm) or three (clip): 8 KB 3.1 against 3.9 us, 128 KB
-// 3.6 against 3.9 us, equal at 512 KB (3.9 us; clip after a fill 8.9 us), behind
-// at 1 MB (clip 12.4 against 9.2 us), where eight SMs cannot read fast enough.
+// launch in place of two (norm) or three (clip), one fp32 tensor in L2, 30 passes
+// in a graph: norm of 8 KB 2.6 against 3.3 us, 128 KB 3.3 against 3.1, equal at
+// 512 KB (3.4), 1 MB 3.9 against 3.6; fill and clip of 8 KB 5.9 against 6.4 us,
+// equal at 128 KB (7.3), 512 KB 8.6 against 8.0, 1 MB 10.7 against 8.1, where eight
+// SMs cannot read fast enough.
 constexpr int kClusterCtas = 8;
 constexpr int kClusterThreads = 1024;
 
@@ -575,8 +580,9 @@ luma_grad_small_kernel(const __grid_constant__ Small t, const FinishArgs a, int 
   });
 }
 
-// The same with a norm for each tensor: in place of three launches (20 tensors
-// with 8 KB 4.6 against 5.8 us, with 512 KB 5.5 against 5.8 us).  A warp leaves a
+// The same with a norm for each tensor: in place of three launches (20 bf16
+// tensors with 8 KB 4.3 against 5.4 us, with 512 KB 5.1 against 5.5, with 1 MB 5.8
+// against 5.5).  A warp leaves a
 // partial at [warp + entry] for every entry that its share touches, as the CTAs
 // of luma_grad_norm_kernel do.
 template <int KIND>

@@ -20,9 +20,15 @@ Tensors are float32, bfloat16 or float16, mixed as they come, dense in memory
 (contiguous in some order of their dimensions), all on one CUDA device, of any
 size (0 included) and alignment.  Work is queued on the device's current
 stream; results are tensors on the device and the same bits on every call with
-the same tensors.  A call may be captured in a CUDA graph; replays then work
-on the captured tensors' memory.  Where a list is empty, the norm is 0 and the
-coefficient that of a norm of 0, on the CPU (with an `inv_scale` on its device).
+the same tensors (the same values at another alignment may differ by the
+rounding of their sums).  All of it is outside autograd: nothing is recorded,
+results carry no gradient, and tensors written in place change their version.
+A function that ``torch.compile`` traces breaks its graph at these calls.  A
+call may be captured in a CUDA graph; replays then work on the captured tensors'
+memory.  Where a list is empty, the norm is 0 and the coefficient that of a norm
+of 0, on the CPU (with an `inv_scale` on its device).
+
+Of a DTensor in a list its local part is read and written.
 """
 
 from __future__ import annotations
@@ -193,8 +199,8 @@ def clip_coef(grads, max_norm: float, norm_type: float = 2.0, *,
     loss scale the grads carry: the norm is then that of the unscaled grads and
     `coef` holds both factors (unscaling and clipping).  `found_inf`, likewise
     one element (and no DTensor), is set to 1 if any element of the grads is
-    inf or NaN, and left alone otherwise.  `error_if_nonfinite` and `process_group` are as in
-    ``grad_norm``."""
+    inf or NaN, and left alone otherwise.  `error_if_nonfinite` and
+    `process_group` are as in ``grad_norm``."""
     kind, bound = _kind(norm_type), _bound(max_norm)
     inv_scale = local_scalar(inv_scale, "inv_scale")
     found_inf = local_flag(found_inf, "found_inf")
@@ -238,8 +244,9 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, *,
 @torch.compiler.disable
 def accumulate_grads_(acc, grads, scale=1.0, *, overwrite: bool = False,
                       norm_type: float | None = None, max_norm: float | None = None):
-    """``acc[i] += scale * grads[i]`` for every i, in one launch: a float32
-    product and a float32 sum per element, rounded to the accumulator's type.
+    """``acc[i] += scale * grads[i]`` for every i, in a launch for each 960 pairs:
+    a float32 product and a float32 sum per element, rounded to the accumulator's
+    type.
     With `overwrite` it is ``acc[i] = scale * grads[i]`` (the first
     micro-batch), whatever `acc` held.
 
@@ -251,9 +258,10 @@ def accumulate_grads_(acc, grads, scale=1.0, *, overwrite: bool = False,
     itself; other overlaps are refused.
 
     With `norm_type` (1, 2 or inf) the norm of the accumulators as they are
-    afterwards is returned, from the same pass; with `max_norm` it is
-    ``(norm, coef)`` as ``clip_coef(acc, max_norm, norm_type or 2)`` gives
-    them.  Otherwise nothing is returned."""
+    afterwards is returned, from the same pass (and a launch that joins its sums);
+    with `max_norm` it is ``(norm, coef)`` as of ``clip_coef(acc, max_norm,
+    norm_type or 2)``, to the rounding of sums in another order.  Otherwise
+    nothing is returned."""
     kind = _lib.NORM_NONE
     if norm_type is not None or max_norm is not None:
         kind = _kind(2.0 if norm_type is None else norm_type)
