@@ -253,7 +253,7 @@ __device__ __forceinline__ double warp_join(int kind, double v) {
 }
 
 // Result in thread 0.  32 warps' values are joined like lanes (a norm of 8 KB
-// 2.90 us, against 3.07 with one thread that takes them one after the other); for
+// of bf16 2.90 us, against 3.07 with one thread that takes them one by one); for
 // 8 warps the shuffles cost the norm kernel two registers too many, and with the
 // spills norms of 10,000 tensors 464 in place of 449 us.
 template <int THREADS>
@@ -537,8 +537,8 @@ __global__ void __launch_bounds__(kThreads) luma_grad_scale_kernel(
 // A small call as a whole: the norm, its results and with `clip` the scaling.
 // One cluster of eight CTAs whose warps share the tiles; the warps' sums are
 // joined in a fixed order, the CTAs' through distributed shared memory.  One
-// launch in place of two (norm) or three (clip), one fp32 tensor in L2, 30 passes
-// in a graph: norm of 8 KB 2.6 against 3.3 us, 128 KB 3.3 against 3.1, equal at
+// launch in place of two (norm) or three (clip), one fp32 tensor that L2 holds, 30
+// passes in a graph: norm of 8 KB 2.6 against 3.3 us, 128 KB 3.3 against 3.1, equal at
 // 512 KB (3.4), 1 MB 3.9 against 3.6; fill and clip of 8 KB 5.9 against 6.4 us,
 // equal at 128 KB (7.3), 512 KB 8.6 against 8.0, 1 MB 10.7 against 8.1, where eight
 // SMs cannot read fast enough.
